@@ -1,0 +1,645 @@
+// Attention over packed sequences (gfx950): out = softmax(scale q k^T) v for sequences of different lengths that lie one
+// behind the other in [tokens, heads, dim] tensors, with grouped heads, causal or not, in fp16, bf16 and fp32.
+//
+// One pass over the keys with a running maximum and sum (softmax in the log2 domain, fp32).  Orientation: S^T = K Q^T puts
+// the keys on the accumulator registers and the query on the lane, so maximum and sum are taken in registers plus one
+// exchange of the lane halves, and the exponentiated tile is already the B operand of O^T += V^T P^T: accumulator element i
+// of lane half h is key 8 (i / 4) + 4 h + i % 4, and the V^T fragments are read in that order of keys.
+//
+// A row is one query of one head; the rows of a key head's group are taken together (row r = query r / group, head
+// r % group), so K and V are read once for the group and a single query still fills `group` rows.
+#include "common.h"
+
+namespace {
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void* lptr_t;
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+
+struct AttArgs {
+  const void *q, *k, *v; void* out; float* sums;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head;
+  const int32_t *starts_q, *starts_k;
+  int tokens_q, tokens_k, sequences, heads, kv_heads, group, dim, causal;
+  float c_log2;                      // |scale| log2(e), positive: masked scores are -inf before it is applied
+  uint32_t q_keep, q_flip;           // bits of q that stay, and that turn: a negative scale negates q, a zero one clears it
+  int clear;                         // rows before the first and behind the last sequence: 1 zero in out, 2 -inf in sums
+  int pairs, replicas, tiles, splits, chunk;    // the grid (launch())
+  float* part_o; float* part_ml;     // partial results of a split key axis
+};
+
+// ---- the three types: a 16-byte fragment, its products, and P
+template <class T> struct Num;
+template <> struct Num<_Float16> {
+  typedef half8 frag;
+  static constexpr bool wide = false;              // (odd(): does a word hold an infinity or NaN?)
+  __device__ static f32x16 mfma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  __device__ static uint32_t pack(float a, float b) { return __builtin_bit_cast(uint32_t, half2v{(_Float16)a, (_Float16)b}); }
+  __device__ static bool odd(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }
+};
+template <> struct Num<__bf16> {
+  typedef bf8 frag;
+  static constexpr bool wide = false;
+  __device__ static f32x16 mfma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  __device__ static uint32_t pack(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf2)); }
+  __device__ static bool odd(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+};
+template <> struct Num<float> {
+  typedef f32x4 frag;
+  static constexpr bool wide = true;
+  __device__ static bool odd(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
+  // four products of two: lane half h holds four neighbouring entries of the contraction
+  __device__ static f32x16 mfma(frag a, frag b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// ---- a tile of keys in LDS: rows of NS steps of 32 bytes (S = 2 NS slots of 16), slots moved by the row so that the reads
+// of neighbouring rows meet different banks: XOR where S is a power of two, rotation otherwise.
+template <int NS> struct Slots {
+  static constexpr int S = 2 * NS, P = 32 * NS;
+  static constexpr bool pow2 = (S & (S - 1)) == 0;
+  static constexpr int gcd16(int x) { return x % 16 == 0 ? 16 : x % 8 == 0 ? 8 : x % 4 == 0 ? 4 : x % 2 == 0 ? 2 : 1; }
+  static constexpr int period = 16 / gcd16(S);
+  // K: 16 rows of one slot column
+  __device__ static int k_turn(int row) { return ((row & 31) / period) % S; }
+  // V, 16-bit transposed reads: four rows of 64 bytes; fp32: two rows, four apart, of 128 bytes
+  template <bool WIDE> __device__ static int v_turn(int row) {
+    if (WIDE) return (S % 4 == 0 && S >= 16) ? 8 * ((row >> 2) & 1) : 0;
+    return S % 16 == 0 ? 4 * (row & 3) : S % 8 == 0 ? 4 * ((row & 3) >> 1) : 0;
+  }
+  __device__ static int place(int slot, int turn) {
+    if (pow2) return slot ^ turn;
+    const int p = slot + turn;
+    return p >= S ? p - S : p;
+  }
+  __device__ static int slot_at(int place_, int turn) {      // the inverse
+    if (pow2) return place_ ^ turn;
+    const int p = place_ - turn;
+    return p < 0 ? p + S : p;
+  }
+};
+
+constexpr float NO_MAX = -3.0e38f;     // of a row that has seen no key: finite, so that no difference of infinities arises
+
+// NS: steps of 32 bytes of a row (dim rounded up); NQ: blocks of 32 rows per wave; WQ x WK waves: over rows x over keys;
+// KB: blocks of 32 keys per wave and tile
+template <class T, int NS, int NQ, int WQ, int WK, int KB>
+struct Shape {
+  static constexpr int W = WQ * WK, THREADS = 64 * W, ROWS = 32 * NQ * WQ, KEYS = 32 * KB * WK;
+  static constexpr int P = 32 * NS, S = 2 * NS, TILE = KEYS * P;           // bytes of K (or V) of a tile
+  static constexpr int E = 16 / (int)sizeof(T);                            // entries of a slot
+  static constexpr int DB = (NS * 2 * E + 31) / 32;                        // blocks of 32 entries of the output
+  static constexpr int BUF = 2 * TILE;
+  static constexpr int JOIN = WK > 1 ? (WK - 1) * WQ * NQ * 64 * (DB * 16 + 2) * 4 : 0;
+  static constexpr int LDS = (2 * BUF + 256 > JOIN ? 2 * BUF + 256 : JOIN);
+  static constexpr int NI = TILE / 1024;                                   // transfers of 64 x 16 bytes per tile of K (or V)
+  static constexpr int NJ = (NI + W - 1) / W;
+};
+
+template <class T, int NS, int NQ, int WQ, int WK, int KB>
+__global__ __launch_bounds__(64 * WQ * WK) void packed_attention_kernel(const AttArgs a) {
+  typedef Shape<T, NS, NQ, WQ, WK, KB> G;
+  typedef Slots<NS> L;
+  typedef Num<T> N;
+  typedef typename N::frag frag;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  constexpr int S = G::S, P = G::P, DB = G::DB, E = G::E;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave % WQ, wk = wave / WQ;
+
+  // block -> (pair of sequence and key head, tile of rows, part of the keys).  Blocks go to the 8 XCDs in turn; each XCD
+  // gets a contiguous eighth of the pairs (pairs are taken `replicas` times to make their number divisible by 8), so the
+  // blocks that share K and V share an L2.
+  const unsigned per_xcd = (unsigned)(a.pairs * a.replicas) / 8;
+  unsigned id = blockIdx.x / 8;
+  const int units = a.tiles * a.splits;
+  const unsigned vp = (blockIdx.x % 8) * per_xcd + id / (unsigned)units;
+  const int unit = (int)(id % (unsigned)units);
+  const int split = unit % a.splits;
+  const int pair = (int)(vp / (unsigned)a.replicas), replica = (int)(vp % (unsigned)a.replicas);
+  const int seq = pair % a.sequences, kvh = pair / a.sequences;
+  const int q0 = min(max(a.starts_q[seq], 0), a.tokens_q), q1 = min(max(a.starts_q[seq + 1], q0), a.tokens_q);
+  const int k0 = min(max(a.starts_k[seq], 0), a.tokens_k), k1 = min(max(a.starts_k[seq + 1], k0), a.tokens_k);
+  const int nq = q1 - q0, nk = k1 - k0, rows = nq * a.group;
+  if (a.clear && unit == 0 && replica == 0) {                              // what lies before the first and behind the last sequence
+    const int width = a.group * a.dim;
+    auto wipe = [&](int first, int last) {
+      for (int64_t i = tid; i < (int64_t)(last - first) * width; i += G::THREADS) {
+        const int64_t t = first + i / width;
+        const int e = (int)(i % width), hh = kvh * a.group + e / a.dim;
+        if (a.clear & 1) static_cast<T*>(a.out)[t * a.o_tok + hh * a.o_head + e % a.dim] = (T)0.f;
+        if ((a.clear & 2) && a.sums && e % a.dim == 0) a.sums[t * a.heads + hh] = -__builtin_inff();
+      }
+    };
+    if (seq == 0) wipe(0, q0);
+    if (seq == a.sequences - 1) wipe(q1, a.tokens_q);
+  }
+  const int split_begin = split * a.chunk;
+  if (split > 0 && split_begin >= nk) return;                              // nothing reads this part (join_kernel)
+  const int split_end = split == a.splits - 1 ? nk : min(nk, split_begin + a.chunk);
+
+  // transfers: lane -> (row, slot) of the tile, the address of the slot's entries behind the tile's first row
+  const uint32_t ks_bytes = (uint32_t)(a.k_tok * sizeof(T)), vs_bytes = (uint32_t)(a.v_tok * sizeof(T));
+  uint32_t koff[G::NJ], voff[G::NJ];
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j) {
+    const int chunk = (wave + G::W * j) * 64 + lane, row = chunk / S, place = chunk - row * S;
+    const int ks = L::slot_at(place, L::k_turn(row)), vs = L::slot_at(place, L::template v_turn<N::wide>(row));
+    koff[j] = ks * E < a.dim ? (uint32_t)row * ks_bytes + ks * 16 : 0x80000000u;      // behind the head: reads as zero
+    voff[j] = vs * E < a.dim ? (uint32_t)row * vs_bytes + vs * 16 : 0x80000000u;
+  }
+  const uint8_t* const kbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.k) + (int64_t)k0 * a.k_tok + kvh * a.k_head);
+  const uint8_t* const vbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.v) + (int64_t)k0 * a.v_tok + kvh * a.v_head);
+  // tile of keys `key` .. : rows behind the sequence read as zero (the descriptor ends with its last entry)
+  auto fetch = [&](int key, int buffer) {
+    const int left = min(nk - key, G::KEYS);
+    const uint64_t kb = (uint64_t)kbase + (uint64_t)key * ks_bytes, vb = (uint64_t)vbase + (uint64_t)key * vs_bytes;
+    const uint32_t kn = (uint32_t)(left - 1) * ks_bytes + a.dim * sizeof(T), vn = (uint32_t)(left - 1) * vs_bytes + a.dim * sizeof(T);
+    const rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(kb), 0, kn, 0x00020000);
+    const rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(vb), 0, vn, 0x00020000);
+    uint8_t* const dst = lds + buffer * G::BUF;
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j) {
+      const int n = wave + G::W * j;
+      if (G::NI % G::W == 0 || n < G::NI) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lptr_t)(dst + n * 1024), 16, (int)koff[j], 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lptr_t)(dst + G::TILE + n * 1024), 16, (int)voff[j], 0, 0, 0);
+      }
+    }
+  };
+
+  for (int tile = (unit / a.splits) * a.replicas + replica; (int64_t)tile * G::ROWS < rows; tile += a.tiles * a.replicas) {
+    const int tile_row = tile * G::ROWS, wave_row = tile_row + wq * 32 * NQ;
+    // keys that a row sees: the first `lim` of its sequence
+    auto limit = [&](int row) {
+      const int i = row / a.group;
+      return a.causal ? min(max(i + nk - nq + 1, 0), nk) : nk;
+    };
+    const int block_last = min(tile_row + G::ROWS, rows) - 1;
+    const int key_end = min(split_end, limit(block_last));
+    const bool active = wave_row < rows;
+    const int lim_least = active ? limit(wave_row) : 0, lim_most = active ? limit(min(wave_row + 32 * NQ, rows) - 1) : 0;
+    int lim[NQ];
+    frag qf[NQ][NS];
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      const int row = wave_row + 32 * b + r, i = row / a.group, hh = kvh * a.group + row - i * a.group;
+      lim[b] = row < rows ? limit(row) : 0;
+      const T* src = static_cast<const T*>(a.q) + (int64_t)(q0 + i) * a.q_tok + (int64_t)hh * a.q_head;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const int d = (2 * s + h) * E;
+        frag z = {};
+        u32x4 w = __builtin_bit_cast(u32x4, row < rows && d < a.dim ? *reinterpret_cast<const frag*>(src + d) : z);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = (w[j] & a.q_keep) ^ a.q_flip;
+        qf[b][s] = __builtin_bit_cast(frag, w);
+      }
+    }
+    f32x16 o[NQ][DB];
+    float m_run[NQ], l_run[NQ];
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      m_run[b] = NO_MAX;
+      l_run[b] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][d][i] = 0.f;
+    }
+
+    // 32 keys, from LDS row `krow` of a tile on; key: the first one's number
+    auto block = [&](const uint8_t* Kt, const uint8_t* Vt, int krow, int key, auto masked_tag) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
+      f32x16 sc[NQ];
+#pragma unroll
+      for (int b = 0; b < NQ; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[b][i] = 0.f;
+      const uint8_t* krp = Kt + (krow + r) * P;
+      const int kt = L::k_turn(r);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const frag kf = *reinterpret_cast<const frag*>(krp + L::place(2 * s + h, kt) * 16);
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) sc[b] = N::mfma(kf, qf[b][s], sc[b]);
+      }
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
+        if constexpr (MASKED) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[b][i] = key + 8 * (i >> 2) + 4 * h + (i & 3) < lim[b] ? sc[b][i] : -__builtin_inff();
+        }
+        float top = sc[b][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[b][i]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float m_new = fmaxf(m_run[b], top * a.c_log2);
+        if (__builtin_amdgcn_ballot_w64(m_new != m_run[b])) {
+          const float corr = __builtin_amdgcn_exp2f(m_run[b] - m_new);
+          l_run[b] *= corr;
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[b][d][i] *= corr;
+          m_run[b] = m_new;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          sc[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], a.c_log2, -m_run[b]));
+          sum += sc[b][i];
+        }
+        l_run[b] += sum;
+      }
+      // O^T += V^T P^T.  only >= 0: that key alone, for the rows that see it (below)
+      auto values = [&](const int only) {
+        constexpr int KS = N::wide ? 16 : 2;
+        auto key_of = [&](int i) { return 8 * (i >> 2) + 4 * h + (i & 3); };
+        frag pf[NQ][2];
+        if constexpr (!N::wide) {
+#pragma unroll
+          for (int b = 0; b < NQ; ++b)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+              u32x4 w;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int i = 8 * ks + 2 * j;
+                w[j] = only < 0 ? N::pack(sc[b][i], sc[b][i + 1]) : N::pack(key_of(i) == only ? sc[b][i] : 0.f, key_of(i + 1) == only ? sc[b][i + 1] : 0.f);
+              }
+              pf[b][ks] = __builtin_bit_cast(frag, w);
+            }
+        }
+        // 16-bit, transposed reads: lane 4 q + p of a 16-lane group addresses key row q, entries 4 p .. of the group's 16, and
+        // gets column (lane & 15) of the 4 x 16 block; the groups take (entries 0 .. 15, 16 .. 31) x (lane halves)
+        const int q = (lane & 15) >> 2, p = lane & 3, g1 = (lane >> 4) & 1;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          f32x16 part[NQ];
+          if (only >= 0) {
+#pragma unroll
+            for (int b = 0; b < NQ; ++b)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) part[b][i] = 0.f;
+          }
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (N::wide) {
+              const int row = krow + key_of(ks);
+              float vf = *reinterpret_cast<const float*>(Vt + row * P + L::place(8 * d + (r >> 2), L::template v_turn<true>(row)) * 16 + (r & 3) * 4);
+              if (only >= 0 && key_of(ks) != only) vf = 0.f;
+#pragma unroll
+              for (int b = 0; b < NQ; ++b) {
+                if (only < 0) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, sc[b][ks], o[b][d], 0, 0, 0);
+                else part[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, key_of(ks) == only ? sc[b][ks] : 0.f, part[b], 0, 0, 0);
+              }
+            } else {
+              u32x4 w;
+#pragma unroll
+              for (int j2 = 0; j2 < 2; ++j2) {
+                const int row = krow + 16 * ks + 8 * j2 + 4 * h + q;
+                const uint8_t* at = Vt + row * P + L::place(4 * d + 2 * g1 + (p >> 1), L::template v_turn<false>(4 * h + q)) * 16 + 8 * (p & 1);
+                const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at)));
+                w[2 * j2] = x[0];
+                w[2 * j2 + 1] = x[1];
+              }
+              if (only >= 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const int i = 8 * ks + 2 * j;
+                  w[j] = key_of(i) == only ? w[j] & 0xffffu : key_of(i + 1) == only ? w[j] & 0xffff0000u : 0u;
+                }
+              }
+              const frag vf = __builtin_bit_cast(frag, w);
+#pragma unroll
+              for (int b = 0; b < NQ; ++b) {
+                if (only < 0) o[b][d] = N::mfma(vf, pf[b][ks], o[b][d]);
+                else part[b] = N::mfma(vf, pf[b][ks], part[b]);
+              }
+            }
+          }
+          if (only >= 0) {
+#pragma unroll
+            for (int b = 0; b < NQ; ++b)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[b][d][i] = key + only < lim[b] ? o[b][d][i] + part[b][i] : o[b][d][i];
+          }
+        }
+      };
+      if constexpr (MASKED) {
+        // A masked score has p = 0, but 0 times an infinity or NaN is NaN: where these 32 values hold one, the keys are taken
+        // one by one and added to the rows that see them alone.
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(Vt + krow * P + j * 1024 + lane * 16);
+          odd |= N::odd(w[0]) | N::odd(w[1]) | N::odd(w[2]) | N::odd(w[3]);
+        }
+        if (__builtin_amdgcn_ballot_w64(odd)) {
+#pragma unroll 1
+          for (int only = 0; only < 32; ++only) values(only);
+          return;
+        }
+      }
+      values(-1);
+    };
+
+    if (key_end > split_begin) fetch(split_begin, 0);
+    int buffer = 0;
+    for (int key = split_begin; key < key_end; key += G::KEYS) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (key + G::KEYS < key_end) fetch(key + G::KEYS, buffer ^ 1);
+      const uint8_t* Kt = lds + buffer * G::BUF;
+      const uint8_t* Vt = Kt + G::TILE;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int krow = (wk * KB + kb) * 32, at = key + krow;
+        if (at >= min(lim_most, key_end)) continue;
+        if (at + 32 <= lim_least && at + 32 <= key_end) block(Kt, Vt, krow, at, std::false_type{});
+        else block(Kt, Vt, krow, at, std::true_type{});
+      }
+      buffer ^= 1;
+    }
+
+    // ---- the lane halves' sums, then the waves that took other keys
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) l_run[b] += __shfl_xor(l_run[b], 32, 64);
+    if constexpr (WK > 1) {
+      __syncthreads();
+      float* const mine = reinterpret_cast<float*>(lds) + (size_t)((wk - 1) * WQ + wq) * NQ * 64 * (DB * 16 + 2);
+      if (wk > 0) {
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) {
+          float* p = mine + b * 64 * (DB * 16 + 2) + lane;
+          p[0] = m_run[b];
+          p[64] = l_run[b];
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[64 * (2 + d * 16 + i)] = o[b][d][i];
+        }
+      }
+      __syncthreads();
+      if (wk == 0) {
+#pragma unroll
+        for (int w = 1; w < WK; ++w)
+#pragma unroll
+          for (int b = 0; b < NQ; ++b) {
+            const float* p = reinterpret_cast<const float*>(lds) + ((size_t)((w - 1) * WQ + wq) * NQ + b) * 64 * (DB * 16 + 2) + lane;
+            const float m_new = fmaxf(m_run[b], p[0]);
+            const float ca = __builtin_amdgcn_exp2f(m_run[b] - m_new), cb = __builtin_amdgcn_exp2f(p[0] - m_new);
+            l_run[b] = l_run[b] * ca + p[64] * cb;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[b][d][i] = o[b][d][i] * ca + p[64 * (2 + d * 16 + i)] * cb;
+            m_run[b] = m_new;
+          }
+      }
+    }
+    if (wk == 0) {
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
+        const int row = wave_row + 32 * b + r;
+        if (row >= rows) continue;
+        const int i = row / a.group, hh = kvh * a.group + row - i * a.group;
+        if (a.splits > 1) {
+          const size_t at = (size_t)split * a.tokens_q * a.heads + (size_t)(q0 + i) * a.heads + hh;
+          float* dst = a.part_o + at * a.dim;
+          if (h == 0) {
+            a.part_ml[2 * at] = m_run[b];
+            a.part_ml[2 * at + 1] = l_run[b];
+          }
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int e = 32 * d + 8 * j + 4 * h;
+              if (e < a.dim) *reinterpret_cast<f32x4*>(dst + e) = f32x4{o[b][d][4 * j], o[b][d][4 * j + 1], o[b][d][4 * j + 2], o[b][d][4 * j + 3]};
+            }
+        } else {
+          const float inv = l_run[b] == 0.f ? 0.f : 1.0f / l_run[b];
+          T* dst = static_cast<T*>(a.out) + (int64_t)(q0 + i) * a.o_tok + (int64_t)hh * a.o_head;
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int e = 32 * d + 8 * j + 4 * h;
+              const float x[4] = {o[b][d][4 * j] * inv, o[b][d][4 * j + 1] * inv, o[b][d][4 * j + 2] * inv, o[b][d][4 * j + 3] * inv};
+              if (e < a.dim) {
+                if constexpr (N::wide) *reinterpret_cast<f32x4*>(dst + e) = f32x4{x[0], x[1], x[2], x[3]};
+                else *reinterpret_cast<u32x2*>(dst + e) = u32x2{N::pack(x[0], x[1]), N::pack(x[2], x[3])};
+              }
+            }
+          if (a.sums && h == 0)
+            a.sums[(size_t)(q0 + i) * a.heads + hh] = l_run[b] == 0.f ? -__builtin_inff() : 0.69314718055994530942f * (m_run[b] + __builtin_amdgcn_logf(l_run[b]));
+        }
+      }
+    }
+    __syncthreads();                 // the next tile's transfers overwrite what these waves may still read
+  }
+}
+
+// Joins the parts of a split key axis: one wave per row, lane -> entries.
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(const AttArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)a.tokens_q * a.heads) return;
+  const int token = (int)(row / a.heads), hh = (int)(row - (int64_t)token * a.heads);
+  // the sequence that holds the token: the first whose (clamped, as above) range does
+  int seq = -1, nk = 0;
+  for (int s0 = 0; s0 < a.sequences && seq < 0; s0 += 64) {
+    const int s = s0 + lane;
+    bool here = false;
+    if (s < a.sequences) {
+      const int q0 = min(max(a.starts_q[s], 0), a.tokens_q), q1 = min(max(a.starts_q[s + 1], q0), a.tokens_q);
+      here = token >= q0 && token < q1;
+    }
+    const unsigned long long m = __builtin_amdgcn_ballot_w64(here);
+    if (m) seq = s0 + __builtin_ctzll(m);
+  }
+  if (seq < 0) return;                                           // behind the last sequence: left as it is
+  const int k0 = min(max(a.starts_k[seq], 0), a.tokens_k);
+  nk = min(max(a.starts_k[seq + 1], k0), a.tokens_k) - k0;
+  const int parts = max(1, min(a.splits, (nk + a.chunk - 1) / a.chunk));
+  const size_t step = (size_t)a.tokens_q * a.heads;
+  float m = NO_MAX;
+  for (int s = 0; s < parts; ++s) m = fmaxf(m, a.part_ml[2 * (s * step + row)]);
+  float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < parts; ++s) {
+    const size_t at = s * step + row;
+    const float c = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - m);
+    l += a.part_ml[2 * at + 1] * c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (lane + 64 * j < a.dim) x[j] += a.part_o[at * a.dim + lane + 64 * j] * c;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  T* dst = static_cast<T*>(a.out) + (int64_t)token * a.o_tok + (int64_t)hh * a.o_head;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (lane + 64 * j < a.dim) dst[lane + 64 * j] = (T)(x[j] * inv);
+  if (a.sums && lane == 0) a.sums[row] = l == 0.f ? -__builtin_inff() : 0.69314718055994530942f * (m + __builtin_amdgcn_logf(l));
+}
+
+// ---- the launch plan: what ac_attention_packed and its workspace size agree on
+struct Plan { int kind, rows, tiles, splits, chunk, keys; };   // kind 0: 256 rows, 1: 128 rows, 2: 32 rows and split keys
+
+template <class T> int plan_steps(int dim) {                    // NS of the instance that holds `dim`
+  const int per = 32 / (int)sizeof(T), need = (dim + per - 1) / per;
+  const int have16[] = {2, 3, 4, 5, 6, 8, 10, 12, 16}, have32[] = {4, 6, 8, 10, 12, 16, 24, 32};
+  if (sizeof(T) == 4) { for (int n : have32) if (n >= need) return n; }
+  else { for (int n : have16) if (n >= need) return n; }
+  return 0;
+}
+
+Plan make_plan(const ac_attention_args* p) {
+  const int group = p->heads / p->kv_heads;
+  const int64_t max_q = min((int64_t)max(p->max_q, 1), max(p->tokens_q, (int64_t)1)), max_k = min((int64_t)max(p->max_k, 1), max(p->tokens_k, (int64_t)1));
+  const int64_t rows = max_q * group, pairs = (int64_t)p->sequences * p->kv_heads;
+  const bool wide = p->type == AC_F32;
+  const int bytes = p->dim * (wide ? 4 : 2);
+  Plan r;
+  r.kind = rows <= 32 ? 2 : (wide || bytes > 256 || pairs * ((rows + 255) / 256) < 2 * ac_device_cus()) ? 1 : 0;
+  r.rows = r.kind == 2 ? 32 : r.kind == 1 ? 128 : 256;
+  r.keys = r.kind == 2 ? (bytes > 512 ? 64 : 128) : 64;
+  r.tiles = (int)((rows + r.rows - 1) / r.rows);
+  // the key axis is split where the rows alone would leave CUs idle, into parts of 512 keys or more
+  const int64_t blocks = pairs * r.tiles, want = 6LL * ac_device_cus();
+  int64_t splits = blocks >= want / 3 ? 1 : min((want + blocks - 1) / blocks, (max_k + 511) / 512);
+  splits = max((int64_t)1, min((int64_t)64, splits));
+  r.chunk = (int)(((max_k + splits - 1) / splits + r.keys - 1) / r.keys * r.keys);
+  r.splits = (int)((max_k + r.chunk - 1) / r.chunk);
+  return r;
+}
+
+template <class T, int NS, int NQ, int WQ, int WK, int KB>
+int launch(const AttArgs& a, hipStream_t stream) {
+  typedef Shape<T, NS, NQ, WQ, WK, KB> G;
+  static unsigned long long done = 0;
+  if (int rc = ac_set_max_lds(reinterpret_cast<const void*>(&packed_attention_kernel<T, NS, NQ, WQ, WK, KB>), G::LDS, &done)) return rc;
+  const int64_t blocks = (int64_t)a.pairs * a.replicas * a.tiles * a.splits;
+  if (blocks >= (1LL << 31)) return ac_fail(AC_EINVAL, "ac_attention_packed: too many blocks");
+  hipLaunchKernelGGL((packed_attention_kernel<T, NS, NQ, WQ, WK, KB>), dim3((unsigned)blocks), dim3(G::THREADS), G::LDS, stream, a);
+  return AC_OK;
+}
+
+template <class T, int NS>
+int launch_kind(const AttArgs& a, int kind, hipStream_t stream) {
+  constexpr bool big = NS * 32 > 256;                            // rows of more than 256 bytes: smaller tiles
+  if constexpr (!Num<T>::wide && !big) {
+    if (kind == 0) return launch<T, NS, 2, 4, 1, 2>(a, stream);
+  }
+  if (kind == 2) {
+    if constexpr (NS * 32 > 512) return launch<T, NS, 1, 1, 1, 1>(a, stream);
+    else if constexpr (big) return launch<T, NS, 1, 1, 2, 1>(a, stream);
+    else return launch<T, NS, 1, 1, 4, 1>(a, stream);
+  }
+  if constexpr (NS * 32 > 512) return launch<T, NS, 1, 4, 1, 1>(a, stream);
+  else return launch<T, NS, 1, 4, 1, big ? 1 : 2>(a, stream);
+}
+
+template <class T>
+int launch_type(const AttArgs& a, int kind, hipStream_t stream) {
+  int rc = AC_EINVAL;
+  if constexpr (sizeof(T) == 4) {
+    switch (plan_steps<T>(a.dim)) {
+      case 4: rc = launch_kind<T, 4>(a, kind, stream); break;
+      case 6: rc = launch_kind<T, 6>(a, kind, stream); break;
+      case 8: rc = launch_kind<T, 8>(a, kind, stream); break;
+      case 10: rc = launch_kind<T, 10>(a, kind, stream); break;
+      case 12: rc = launch_kind<T, 12>(a, kind, stream); break;
+      case 16: rc = launch_kind<T, 16>(a, kind, stream); break;
+      case 24: rc = launch_kind<T, 24>(a, kind, stream); break;
+      case 32: rc = launch_kind<T, 32>(a, kind, stream); break;
+    }
+  } else {
+    switch (plan_steps<T>(a.dim)) {
+      case 2: rc = launch_kind<T, 2>(a, kind, stream); break;
+      case 3: rc = launch_kind<T, 3>(a, kind, stream); break;
+      case 4: rc = launch_kind<T, 4>(a, kind, stream); break;
+      case 5: rc = launch_kind<T, 5>(a, kind, stream); break;
+      case 6: rc = launch_kind<T, 6>(a, kind, stream); break;
+      case 8: rc = launch_kind<T, 8>(a, kind, stream); break;
+      case 10: rc = launch_kind<T, 10>(a, kind, stream); break;
+      case 12: rc = launch_kind<T, 12>(a, kind, stream); break;
+      case 16: rc = launch_kind<T, 16>(a, kind, stream); break;
+    }
+  }
+  if (rc != AC_OK) return rc;
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)a.tokens_q * a.heads;
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
+  }
+  return AC_OK;
+}
+
+int check(const ac_attention_args* p) {
+  AC_REQUIRE(p, "ac_attention_packed: null arguments");
+  AC_REQUIRE(p->type == AC_F32 || p->type == AC_F16 || p->type == AC_BF16, "ac_attention_packed: unknown type %d", p->type);
+  AC_REQUIRE(p->heads >= 1 && p->kv_heads >= 1 && p->heads % p->kv_heads == 0, "ac_attention_packed: %d heads cannot share %d key heads", p->heads, p->kv_heads);
+  AC_REQUIRE(p->dim >= 8 && p->dim <= 256 && p->dim % 8 == 0, "ac_attention_packed: head dim %d must be a multiple of 8, 8 .. 256", p->dim);
+  AC_REQUIRE(p->sequences >= 0 && p->tokens_q >= 0 && p->tokens_k >= 0, "ac_attention_packed: negative count");
+  AC_REQUIRE(p->tokens_q * (int64_t)(p->heads / p->kv_heads) + 256 < (1LL << 31) && p->tokens_k + 256 < (1LL << 31) && p->tokens_q * (int64_t)p->heads < (1LL << 32),
+             "ac_attention_packed: too many tokens");
+  AC_REQUIRE(p->scale - p->scale == 0.f, "ac_attention_packed: the scale is not finite");
+  AC_REQUIRE((int64_t)p->sequences * p->kv_heads < (1LL << 27), "ac_attention_packed: too many sequences");
+  return AC_OK;
+}
+
+}  // namespace
+
+extern "C" size_t ac_attention_packed_workspace_bytes(const ac_attention_args* p) {
+  if (check(p) != AC_OK || p->sequences == 0 || p->tokens_q == 0) return 0;
+  const Plan r = make_plan(p);
+  if (r.splits <= 1) return 0;
+  const size_t rows = (size_t)r.splits * p->tokens_q * p->heads;
+  return align_up(rows * p->dim * 4, 256) + align_up(rows * 8, 256);
+}
+
+extern "C" int ac_attention_packed(const ac_attention_args* p, void* ws, size_t ws_bytes, void* stream_) {
+  if (int rc = check(p)) return rc;
+  if (p->sequences == 0 || p->tokens_q == 0) return AC_OK;
+  AC_REQUIRE(p->q && p->out && p->starts_q && p->starts_k && (p->tokens_k == 0 || (p->k && p->v)), "ac_attention_packed: null pointer");
+  AC_REQUIRE((((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out) & 15) == 0 && (((uintptr_t)p->starts_q | (uintptr_t)p->starts_k | (uintptr_t)p->sums) & 3) == 0,
+             "ac_attention_packed: q, k, v and out must be 16-byte aligned");
+  const int64_t strides[] = {p->q_token, p->q_head, p->k_token, p->k_head, p->v_token, p->v_head, p->out_token, p->out_head};
+  const int entries = p->type == AC_F32 ? 4 : 8;
+  for (int64_t s : strides) AC_REQUIRE(s >= 0 && s % entries == 0, "ac_attention_packed: strides must be non-negative multiples of 16 bytes");
+  AC_REQUIRE(p->k_token < (1 << 20) && p->v_token < (1 << 20), "ac_attention_packed: a key's stride must stay under 2^20 entries");
+  const Plan r = make_plan(p);
+  const size_t need = ac_attention_packed_workspace_bytes(p);
+  if (need && (!ws || ws_bytes < need)) return ac_fail(AC_EWORKSPACE, "ac_attention_packed: workspace %zu < %zu", ws ? ws_bytes : (size_t)0, need);
+  AC_REQUIRE(!need || ((uintptr_t)ws & 15) == 0, "ac_attention_packed: the workspace must be 16-byte aligned");
+  AttArgs a;
+  a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.sums = p->sums;
+  a.q_tok = p->q_token; a.q_head = p->q_head; a.k_tok = p->k_token; a.k_head = p->k_head;
+  a.v_tok = p->v_token; a.v_head = p->v_head; a.o_tok = p->out_token; a.o_head = p->out_head;
+  a.starts_q = p->starts_q; a.starts_k = p->starts_k;
+  a.tokens_q = (int)p->tokens_q; a.tokens_k = (int)p->tokens_k; a.sequences = p->sequences; a.heads = p->heads; a.kv_heads = p->kv_heads;
+  a.group = p->heads / p->kv_heads; a.dim = p->dim; a.causal = p->causal; a.clear = p->clear;
+  a.c_log2 = p->scale == 0.f ? 1.f : fabsf(p->scale) * 1.44269504088896340736f;
+  a.q_keep = p->scale == 0.f ? 0u : ~0u;
+  a.q_flip = p->scale < 0.f ? (p->type == AC_F32 ? 0x80000000u : 0x80008000u) : 0u;
+  a.pairs = p->sequences * p->kv_heads;
+  a.replicas = a.pairs % 8 == 0 ? 1 : a.pairs % 4 == 0 ? 2 : a.pairs % 2 == 0 ? 4 : 8;
+  a.tiles = (r.tiles + a.replicas - 1) / a.replicas; a.splits = r.splits; a.chunk = r.chunk;
+  a.part_o = static_cast<float*>(ws);
+  a.part_ml = need ? reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + align_up((size_t)r.splits * p->tokens_q * p->heads * p->dim * 4, 256)) : nullptr;
+  int rc = p->type == AC_F32 ? launch_type<float>(a, r.kind, as_stream(stream_))
+         : p->type == AC_F16 ? launch_type<_Float16>(a, r.kind, as_stream(stream_)) : launch_type<__bf16>(a, r.kind, as_stream(stream_));
+  if (rc != AC_OK) return rc;
+  return ac_check_launch("ac_attention_packed");
+}

@@ -6,6 +6,7 @@ fallback and no torch-op fallback: a missing library, a CPU tensor or a non-zero
 return code raises.
 """
 import ctypes
+import math
 import os
 import threading
 
@@ -29,6 +30,22 @@ class BlockWeights(_c.Structure):
     """struct ac_block_weights (include/ac_hip.h)."""
     _fields_ = [(n, _vp) for n in ("ln1_w", "ln1_b", "qkv_w", "qkv_b", "proj_w", "proj_b",
                                    "ln2_w", "ln2_b", "fc1_w", "fc1_b", "fc2_w", "fc2_b")]
+
+
+class RotaryArgs(_c.Structure):
+    """struct ac_rotary_args (include/ac_hip.h)."""
+    _fields_ = [("src", _vp * 2), ("dst", _vp * 2), ("src_token", _i64 * 2), ("src_head", _i64 * 2), ("dst_token", _i64 * 2),
+                ("dst_head", _i64 * 2), ("heads", _i * 2), ("positions", _vp), ("position_axis", _i64), ("positions64", _i),
+                ("frequencies", _vp), ("tokens", _i64), ("type", _i), ("layout", _i), ("dim", _i), ("part", _i), ("offset", _i),
+                ("axes", _i), ("inverse", _i), ("amplitude", _f)]
+
+
+class AttentionArgs(_c.Structure):
+    """struct ac_attention_args (include/ac_hip.h)."""
+    _fields_ = ([(n, _vp) for n in ("q", "k", "v", "out", "sums")]
+                + [(n, _i64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "out_token", "out_head")]
+                + [("starts_q", _vp), ("starts_k", _vp), ("tokens_q", _i64), ("tokens_k", _i64)]
+                + [(n, _i) for n in ("sequences", "heads", "kv_heads", "dim", "max_q", "max_k", "causal", "clear", "type")] + [("scale", _f)])
 
 
 ABI_VERSION = 600      # include/ac_hip.h AC_ABI_VERSION
@@ -79,6 +96,9 @@ SIGNATURES = {
     "ac_pdist": (_i, [_vp, _i64, _i, _vp, _vp]),
     "ac_ward_workspace_bytes": (_sz, [_i64]),
     "ac_ward_linkage": (_i, [_vp, _i64, _vp, _vp, _vp, _sz, _vp]),
+    "ac_rotary": (_i, [_c.POINTER(RotaryArgs), _vp]),
+    "ac_attention_packed_workspace_bytes": (_sz, [_c.POINTER(AttentionArgs)]),
+    "ac_attention_packed": (_i, [_c.POINTER(AttentionArgs), _vp, _sz, _vp]),
     "ac_cluster_scores": (_i, [_vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp]),
 }
 
@@ -821,3 +841,239 @@ def cluster_scores(labels_true, labels_pred, k_true, k_pred):
         raise ValueError("a label lies outside [0, k)")
     s = scores.cpu()
     return float(s[0]), float(s[1]), C.cpu().numpy()
+
+
+# ---------------------------------------------------------- packed sequences
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+_LAYOUTS = {"half": ROTARY_HALF, "interleaved": ROTARY_INTERLEAVED}
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _heads(t, name, like=None):
+    """A [tokens, heads, dim] device tensor with neighbouring entries, of `like`'s type, device and dim."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError("%s must be a tensor on the HIP device (got %s); the MI355X path has no CPU fallback"
+                           % (name, getattr(t, "device", type(t))))
+    if t.dim() != 3:
+        raise ValueError("%s must be [tokens, heads, dim], got %s" % (name, tuple(t.shape)))
+    if t.dtype not in _TYPES:
+        raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError("%s: the entries of a head must be neighbours (stride 1), got stride %d" % (name, t.stride(2)))
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise RuntimeError("%s requires a gradient: this operator has no backward pass (use torch.no_grad() or detach())" % name)
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise TypeError("%s is %s, but q is %s" % (name, t.dtype, like.dtype))
+        if t.device != like.device:
+            raise ValueError("%s is on %s, but q is on %s" % (name, t.device, like.device))
+        if t.shape[2] != like.shape[2]:
+            raise ValueError("%s has heads of %d, but q of %d" % (name, t.shape[2], like.shape[2]))
+    return t
+
+
+def _whole(t, dtypes, name, device):
+    """A contiguous device tensor of one of `dtypes` on `device`."""
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise RuntimeError("%s must be a tensor on %s (got %s)" % (name, device, getattr(t, "device", type(t))))
+    if t.dtype not in dtypes:
+        raise TypeError("%s must be %s, got %s" % (name, " or ".join(str(d) for d in dtypes), t.dtype))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+    return t
+
+
+def _span(t):
+    """[first, last) byte of what a tensor's entries lie in (empty: the same number twice)."""
+    first = t.data_ptr()
+    return first, first if t.numel() == 0 else first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _same_view(a, b):
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and all(n <= 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
+
+
+def _apart(a, b):
+    """No entry of `a` is one of `b`: their spans do not meet, or both are head ranges of the same rows (slices of one buffer)."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    if a.stride(0) != b.stride(0) or a.element_size() != b.element_size():
+        return False
+    pitch = a.stride(0) * a.element_size()
+    rows = [(lambda s: s[1] - s[0])(_span(t[:1])) for t in (a, b)]           # bytes of one token's entries
+    d = (b0 - a0) % pitch if pitch else 0
+    return pitch > 0 and d >= rows[0] and d + rows[1] <= pitch
+
+
+def _writable(t, name):
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) or not _rows_apart(t):
+        raise ValueError("%s: its entries overlap each other (strides %s)" % (name, tuple(t.stride())))
+
+
+def _rows_apart(t):
+    reach = 1
+    for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda x: x[1]):
+        if s < reach:
+            return False
+        reach = s * (n - 1) + reach
+    return True
+
+
+def sequence_starts(lengths, device):
+    """(starts int32 [sequences + 1] on `device`, the longest length) of a list of lengths, as attention_packed takes them."""
+    lengths = [int(n) for n in lengths]
+    if any(n < 0 for n in lengths):
+        raise ValueError("negative sequence length in %s" % lengths)
+    starts = [0]
+    for n in lengths:
+        starts.append(starts[-1] + n)
+    if starts[-1] >= 1 << 31:
+        raise ValueError("%d tokens do not fit int32 starts" % starts[-1])
+    return torch.tensor(starts, dtype=torch.int32).to(device), max(lengths, default=0)
+
+
+def rotary_frequencies(part, base=10000.0, axes=1, factor=1.0, original=None, low=1.0, high=32.0, device="cpu"):
+    """Radians per position of the pairs of a rotary part, fp64 [axes, part / 2 / axes]: base ** (-i / pairs).
+
+    factor > 1 stretches a context `original` positions long: pairs that turn fewer than `low` times over it are slowed by
+    the factor, those that turn more than `high` times are kept, those between are mixed linearly in their number of turns.
+    original=None slows every pair (plain position interpolation)."""
+    if axes < 1 or part < 2 or part % (2 * axes):
+        raise ValueError("part=%d must be a positive multiple of 2 * axes (%d)" % (part, 2 * axes))
+    if not base > 0 or not factor > 0 or not high > low:
+        raise ValueError("base and factor must be positive, high above low")
+    pairs = part // 2 // axes
+    f = float(base) ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+    if factor != 1.0:
+        keep = torch.zeros_like(f)
+        if original is not None:
+            keep = ((original * f / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+    return f.repeat(axes, 1).to(device)
+
+
+def rotary(q, k, positions, frequencies, layout="half", offset=0, amplitude=1.0, inverse=False, out_q=None, out_k=None):
+    """Rotary positions of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (or None): pair i of a head turns by
+    position * frequencies[i] in entries offset .. offset + part, the rest is copied (include/ac_hip.h ac_rotary).
+
+    positions: int32 / int64 [tokens] or [axes, tokens]; frequencies: fp64 [axes, part / 2 / axes] (or [part / 2]) on the
+    device (rotary_frequencies).  inverse=True turns back by the same angles (the transpose of the map: its gradient).
+    out_q / out_k: where to write; q / k themselves turn in place.  Returns out_q, or (out_q, out_k) with k."""
+    _heads(q, "q")
+    if layout not in _LAYOUTS:
+        raise ValueError("layout must be 'half' or 'interleaved', got %r" % (layout,))
+    tokens, heads, dim = q.shape
+    if k is not None:
+        _heads(k, "k", q)
+        if k.shape[0] != tokens:
+            raise ValueError("k has %d tokens, but q has %d" % (k.shape[0], tokens))
+    elif out_k is not None:
+        raise ValueError("out_k without k")
+    _whole(frequencies, (torch.float64,), "frequencies", q.device)
+    if frequencies.dim() not in (1, 2):
+        raise ValueError("frequencies must be [axes, pairs] or [pairs], got %s" % (tuple(frequencies.shape),))
+    axes = frequencies.shape[0] if frequencies.dim() == 2 else 1
+    _whole(positions, (torch.int32, torch.int64), "positions", q.device)
+    if tuple(positions.shape) not in ((axes, tokens),) + (((tokens,),) if axes == 1 else ()):
+        raise ValueError("positions must be [%d, %d]%s, got %s" % (axes, tokens, " or [%d]" % tokens if axes == 1 else "", tuple(positions.shape)))
+    a = RotaryArgs()
+    outs = []
+    for i, (x, out, name) in enumerate(((q, out_q, "out_q"), (k, out_k, "out_k"))):
+        if x is None:
+            continue
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        else:
+            _heads(out, name, q)
+            if out.shape != x.shape:
+                raise ValueError("%s must be %s, got %s" % (name, tuple(x.shape), tuple(out.shape)))
+            _writable(out, name)
+            for other, other_name in ((q, "q"), (k, "k")):
+                if other is not None and not _apart(out, other) and not (other is x and _same_view(out, x)):
+                    raise ValueError("%s overlaps %s" % (name, other_name))
+            if outs and not _apart(out, outs[0]):
+                raise ValueError("out_k overlaps out_q")
+        outs.append(out)
+        a.src[i], a.dst[i], a.heads[i] = x.data_ptr(), out.data_ptr(), x.shape[1]
+        a.src_token[i], a.src_head[i], a.dst_token[i], a.dst_head[i] = x.stride(0), x.stride(1), out.stride(0), out.stride(1)
+    a.positions, a.position_axis, a.positions64 = positions.data_ptr(), tokens, int(positions.dtype == torch.int64)
+    a.frequencies = frequencies.data_ptr()
+    a.tokens, a.type, a.layout, a.dim, a.part = tokens, _TYPES[q.dtype], _LAYOUTS[layout], dim, 2 * frequencies.numel()
+    a.offset, a.axes, a.inverse, a.amplitude = int(offset), axes, int(bool(inverse)), float(amplitude)
+    if heads == 0 or (k is not None and k.shape[1] == 0):
+        raise ValueError("q and k need a head each")
+    with torch.cuda.device(q.device):
+        _check(lib().ac_rotary(_c.byref(a), _stream()))
+    return outs[0] if k is None else (outs[0], outs[1])
+
+
+def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, causal=False, scale=None, out=None, want_sums=False):
+    """softmax(scale q k^T) v over packed sequences (include/ac_hip.h ac_attention_packed).
+
+    q [tokens, heads, dim], k and v [key tokens, kv_heads, dim], heads a multiple of kv_heads; float32, float16 or bfloat16;
+    dim a multiple of 8 up to 256.  Sequence s is the rows starts_q[s] .. starts_q[s + 1] of q and starts_k[s] .. of k and v
+    (int32 [sequences + 1] on the device; sequence_starts makes them); starts_k=None: the same as starts_q.  max_q / max_k: upper
+    bounds of the lengths - they shape the launch and never the result; None takes the number of tokens.  causal: query i of n
+    sees key j of m where j <= i + m - n.  A row that sees no key is zero; rows outside every sequence are left as they
+    were in `out` (without `out`: zero).  scale: 1 / sqrt(dim) unless given.  want_sums: also the fp32 [tokens, heads] logarithm of
+    each row's sum of exponentials (-inf for a row that sees no key, and outside every sequence).
+    Tensors whose heads do not start at multiples of 16 bytes are copied first."""
+    _heads(q, "q")
+    _heads(k, "k", q)
+    _heads(v, "v", q)
+    tokens, heads, dim = q.shape
+    if k.shape != v.shape:
+        raise ValueError("k is %s, but v is %s" % (tuple(k.shape), tuple(v.shape)))
+    if starts_k is None:
+        starts_k = starts_q
+        if k.shape[0] != tokens:
+            raise ValueError("k has %d tokens and q %d: starts_k is needed" % (k.shape[0], tokens))
+    for t, name in ((starts_q, "starts_q"), (starts_k, "starts_k")):
+        _whole(t, (torch.int32,), name, q.device)
+        if t.dim() != 1 or t.shape[0] < 1:
+            raise ValueError("%s must be [sequences + 1], got %s" % (name, tuple(t.shape)))
+    if starts_q.shape != starts_k.shape:
+        raise ValueError("starts_q speaks of %d sequences, starts_k of %d" % (starts_q.shape[0] - 1, starts_k.shape[0] - 1))
+    clear = out is None
+    if clear:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _heads(out, "out", q)
+        if out.shape != q.shape:
+            raise ValueError("out must be %s, got %s" % (tuple(q.shape), tuple(out.shape)))
+        _writable(out, "out")
+        for t, name in ((q, "q"), (k, "k"), (v, "v")):
+            if not _apart(out, t):
+                raise ValueError("out overlaps %s" % name)
+        if not _aligned(out):
+            raise ValueError("out: every head must start at a multiple of 16 bytes")
+    q, k, v = (t if _aligned(t) else t.contiguous() if _aligned(t.contiguous()) else t.clone() for t in (q, k, v))
+    sums = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if want_sums else None
+    if starts_q.shape[0] == 1:                             # no sequence at all
+        if clear:
+            out.zero_()
+        if want_sums:
+            sums.fill_(-math.inf)
+        return (out, sums) if want_sums else out
+    a = AttentionArgs()
+    a.q, a.k, a.v, a.out, a.sums = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), sums.data_ptr() if want_sums else None
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        for i, what in enumerate(("token", "head")):        # the stride of an axis of one says nothing
+            setattr(a, "%s_%s" % (name, what), t.stride(i) if t.shape[i] > 1 else 0)
+    a.starts_q, a.starts_k, a.sequences = starts_q.data_ptr(), starts_k.data_ptr(), starts_q.shape[0] - 1
+    a.tokens_q, a.tokens_k, a.heads, a.kv_heads, a.dim = tokens, k.shape[0], heads, k.shape[1], dim
+    a.max_q, a.max_k = tokens if max_q is None else int(max_q), k.shape[0] if max_k is None else int(max_k)
+    a.causal, a.clear, a.type, a.scale = int(bool(causal)), int(clear) | 2 * int(want_sums), _TYPES[q.dtype], float(dim ** -0.5 if scale is None else scale)
+    with torch.cuda.device(q.device):
+        n = lib().ac_attention_packed_workspace_bytes(_c.byref(a))
+        # of its own for every call: two graphs captured on one stream must not share the parts of a split key axis
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        _check(lib().ac_attention_packed(_c.byref(a), ws.data_ptr() if n else None, n, _stream()))
+    return (out, sums) if want_sums else out
+
+
+def _aligned(t):
+    """Every head starts at a multiple of 16 bytes, as the kernels load them."""
+    size = t.element_size()
+    return t.data_ptr() % 16 == 0 and all(n <= 1 or s * size % 16 == 0 for n, s in zip(t.shape[:2], t.stride()[:2]))

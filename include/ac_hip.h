@@ -323,6 +323,57 @@ int ac_ward_linkage(const double* condensed, int64_t n, double* Z, int32_t* bad_
 int ac_cluster_scores(const int32_t* labels_true, const int32_t* labels_pred, int64_t n, int k_true, int k_pred,
                       uint64_t* contingency, double* scores, int32_t* bad_label_flag, void* stream);
 
+/* --------------------------------------------------------- packed sequences */
+
+/* Operators on sequences of different lengths that lie one behind the other in [tokens, heads, dim] tensors (images of their
+ * own sizes, prompts of their own lengths): sequence s is the rows starts[s] .. starts[s + 1].  Strides are in entries, the
+ * entries of a head are neighbours.  They need no reference counterpart: the reference's ViT (vision_transformer.py:80-92)
+ * takes one length per batch and learned positions.  Adding them left every earlier entry point as it was, and a binding
+ * that misses one fails on its name, so AC_ABI_VERSION stays. */
+#define AC_F32 0
+#define AC_F16 1
+#define AC_BF16 2
+
+#define AC_ROTARY_HALF 0        /* pair i = entries (i, i + part / 2) of the turned part */
+#define AC_ROTARY_INTERLEAVED 1 /* pair i = entries (2 i, 2 i + 1) */
+
+/* Rotary positions: pair i of each head turns by angle = position * frequencies[i]: (a, b) -> amplitude * (a cos - b sin,
+ * b cos + a sin); inverse != 0 turns back (the transpose of the map: what a gradient needs).  Entries offset .. offset + part
+ * of a head turn, the others are copied.  frequencies: fp64 [part / 2], radians per position; pairs of axis x, x = i / (part / 2
+ * / axes), use the positions at x * position_axis.  Positions are int32, or int64 with positions64 != 0, and may be negative;
+ * angles are formed in fp64.  src / dst / heads [0] is q, [1] is k (heads[1] = 0: q alone).  dst may be src with the same
+ * strides, and must not overlap it otherwise. */
+typedef struct ac_rotary_args {
+  const void* src[2]; void* dst[2];
+  int64_t src_token[2], src_head[2], dst_token[2], dst_head[2];
+  int32_t heads[2];
+  const void* positions; int64_t position_axis; int32_t positions64;
+  const double* frequencies;
+  int64_t tokens;
+  int32_t type, layout, dim, part, offset, axes, inverse;
+  float amplitude;
+} ac_rotary_args;
+int ac_rotary(const ac_rotary_args* args, void* stream);
+
+/* Attention over packed sequences: out[t, h] = sum_j p_j v[j, g], p = softmax(scale * q[t, h] . k[j, g]) over the keys of the
+ * token's own sequence, g = h / (heads / kv_heads).  causal: query i of n sees key j of m where j <= i + m - n (the last query
+ * sees every key).  A row that sees no key is zero and its log-sum -inf; a key that a row does not see cannot touch it,
+ * whatever it holds.  Rows before the first and behind the last sequence are left as they are; clear
+ * & 1 makes them zero in out, clear & 2 -inf in sums.
+ * starts_q, starts_k: int32 [sequences + 1] on the device, clamped there to 0 .. tokens.  max_q, max_k: upper bounds of the
+ * lengths, used for the launch's shape alone (too small a bound costs time, not rows).  sums (nullable): fp32 [tokens_q,
+ * heads], the natural logarithm of each row's sum of exponentials.  out must not overlap q, k or v. */
+typedef struct ac_attention_args {
+  const void *q, *k, *v; void* out; float* sums;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  const int32_t *starts_q, *starts_k;
+  int64_t tokens_q, tokens_k;
+  int32_t sequences, heads, kv_heads, dim, max_q, max_k, causal, clear, type;
+  float scale;
+} ac_attention_args;
+size_t ac_attention_packed_workspace_bytes(const ac_attention_args* args);
+int ac_attention_packed(const ac_attention_args* args, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
