@@ -1,0 +1,419 @@
+// Layer norm of rows, forward and backward (gfx950), for fp32, fp16 and bf16 rows of any width.
+//
+// forward   y = (x - mean) rstd w + b,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+// backward  g = dy w, u = (x - mean) rstd:  dx = rstd (g - mean(g) - u mean(g u)),  dw = sum_rows dy u,  db = sum_rows dy
+// Statistics, sums and gradients of the weights are fp32; the variance is taken from the differences (two passes over
+// registers), and each result is rounded to its type once.
+//
+// Bound: memory.  A row lives in the registers of the wave or block that owns it, so x (and dy) are read once; a block of the
+// backward pass walks over many rows with its share of dw and db in registers, and a second kernel adds the blocks' shares
+// in a fixed order (no atomics: the same bits every time).
+#include <initializer_list>
+
+#include "common.h"
+
+namespace {
+
+struct NormArgs {
+  const void *x, *dy, *w, *b; void *y, *dx;
+  int64_t x_row, dy_row, y_row, dx_row;          // strides in entries
+  float *mean, *rstd; const float *mean_in, *rstd_in;
+  float* part; int blocks;                       // backward: [blocks][2][C], dw then db
+  void *dw, *db;
+  int64_t rows; int C, w32; float eps;
+};
+
+template <class T, int VEC> struct Pack { typedef T type __attribute__((ext_vector_type(VEC))); };
+template <class T> struct Pack<T, 1> { typedef T type; };
+template <class T, int VEC>
+__device__ inline void load(const T* p, float* v) {
+  typename Pack<T, VEC>::type x = *reinterpret_cast<const typename Pack<T, VEC>::type*>(p);
+  if constexpr (VEC == 1) v[0] = (float)x;
+  else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = (float)x[j];
+  }
+}
+template <class T, int VEC>
+__device__ inline void store(T* p, const float* v) {
+  typename Pack<T, VEC>::type x;
+  if constexpr (VEC == 1) x = (T)v[0];
+  else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = (T)v[j];
+  }
+  *reinterpret_cast<typename Pack<T, VEC>::type*>(p) = x;
+}
+// VEC weights in the rows' type or fp32 (VEC of the rows: 16 bytes at most of theirs, 32 of fp32)
+template <class T, int VEC>
+__device__ inline void load_w(const void* p, int w32, int at, float* v) {
+  if (w32) {
+    constexpr int Q = VEC < 4 ? VEC : 4;
+#pragma unroll
+    for (int j = 0; j < VEC; j += Q) load<float, Q>(static_cast<const float*>(p) + at + j, v + j);
+  } else load<T, VEC>(static_cast<const T*>(p) + at, v);
+}
+
+// sum over the W waves that share a row: [2] values
+template <int W>
+__device__ inline void row_sum(float& a, float& b, float (*box)[2], int wave) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if constexpr (W > 1) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) { box[wave][0] = a; box[wave][1] = b; }
+    __syncthreads();
+    a = b = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) { a += box[i][0]; b += box[i][1]; }
+  }
+}
+
+// N chunks of VEC entries per thread, W waves per row; 4 / W rows (at least one) per block at a time
+template <class T, int VEC, int N, int W>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_forward_kernel(const NormArgs a) {
+  constexpr int R = W >= 4 ? 1 : 4 / W;
+  __shared__ float box[W][2];
+  const int tid = threadIdx.x, wave = tid >> 6, t = R == 1 ? tid : tid % (64 * W);
+  const int64_t row = (int64_t)blockIdx.x * R + (R == 1 ? 0 : wave / W);
+  if (row >= a.rows) return;                      // (whole waves; R > 1 only with W == 1, where no barrier follows)
+  const T* x = static_cast<const T*>(a.x) + row * a.x_row;
+  const int chunks = a.C / VEC;
+  float v[N][VEC];
+  float s = 0.f, zero = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = t + 64 * W * i;
+    if (c < chunks) {
+      load<T, VEC>(x + c * VEC, v[i]);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s += v[i][j];
+    }
+  }
+  row_sum<W>(s, zero, box, wave);
+  const float mean = s / (float)a.C;
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (t + 64 * W * i < chunks) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) { v[i][j] -= mean; q += v[i][j] * v[i][j]; }
+    }
+  }
+  row_sum<W>(q, zero, box, wave);
+  const float rstd = 1.0f / sqrtf(q / (float)a.C + a.eps);
+  T* y = static_cast<T*>(a.y) + row * a.y_row;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = t + 64 * W * i;
+    if (c < chunks) {
+      float w[VEC], b[VEC], o[VEC];
+      if (a.w) load_w<T, VEC>(a.w, a.w32, c * VEC, w);
+      if (a.b) load_w<T, VEC>(a.b, a.w32, c * VEC, b);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        o[j] = v[i][j] * rstd;
+        if (a.w) o[j] *= w[j];
+        if (a.b) o[j] += b[j];
+      }
+      store<T, VEC>(y + c * VEC, o);
+    }
+  }
+  if (t == 0 && a.mean) { a.mean[row] = mean; a.rstd[row] = rstd; }
+}
+
+template <class T, int VEC, int N, int W>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_backward_kernel(const NormArgs a) {
+  constexpr int R = W >= 4 ? 1 : 4 / W;           // rows in flight per block
+  __shared__ float box[W][2];
+  const int tid = threadIdx.x, wave = tid >> 6, t = R == 1 ? tid : tid % (64 * W), sub = R == 1 ? 0 : wave / W;
+  const int chunks = a.C / VEC;
+  float w[N][VEC], dw[N][VEC], db[N][VEC];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = t + 64 * W * i;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { w[i][j] = 1.f; dw[i][j] = db[i][j] = 0.f; }
+    if (a.w && c < chunks) load_w<T, VEC>(a.w, a.w32, c * VEC, w[i]);
+  }
+  const float inv = 1.0f / (float)a.C;
+  for (int64_t row = (int64_t)blockIdx.x * R + sub; row < a.rows; row += (int64_t)gridDim.x * R) {
+    const T* x = static_cast<const T*>(a.x) + row * a.x_row;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.dy_row;
+    const float mean = a.mean_in[row], rstd = a.rstd_in[row];
+    float u[N][VEC], g[N][VEC], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = t + 64 * W * i;
+      if (c < chunks) {
+        load<T, VEC>(x + c * VEC, u[i]);
+        load<T, VEC>(dy + c * VEC, g[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (t + 64 * W * i < chunks) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          u[i][j] = (u[i][j] - mean) * rstd;
+          dw[i][j] += g[i][j] * u[i][j];
+          db[i][j] += g[i][j];
+          g[i][j] *= w[i][j];
+          s1 += g[i][j];
+          s2 += g[i][j] * u[i][j];
+        }
+      }
+    }
+    if (a.dx) {
+      row_sum<W>(s1, s2, box, wave);
+      s1 *= inv;
+      s2 *= inv;
+      T* dx = static_cast<T*>(a.dx) + row * a.dx_row;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = t + 64 * W * i;
+        if (c < chunks) {
+          float o[VEC];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) o[j] = rstd * (g[i][j] - s1 - u[i][j] * s2);
+          store<T, VEC>(dx + c * VEC, o);
+        }
+      }
+    }
+  }
+  if (!a.part) return;
+  float* p = a.part + ((size_t)blockIdx.x * R + sub) * 2 * a.C;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = t + 64 * W * i;
+    if (c < chunks) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) { p[c * VEC + j] = dw[i][j]; p[a.C + c * VEC + j] = db[i][j]; }
+    }
+  }
+}
+
+// Rows too wide for registers: one block per row, x read again for each pass (the second and third from a cache)
+template <class T>
+__global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const NormArgs a) {
+  __shared__ float box[16][2];
+  const int wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_row;
+  float s = 0.f, q = 0.f, zero = 0.f;
+  for (int c = threadIdx.x; c < a.C; c += 1024) s += (float)x[c];
+  row_sum<16>(s, zero, box, wave);
+  const float mean = s / (float)a.C;
+  for (int c = threadIdx.x; c < a.C; c += 1024) { const float d = (float)x[c] - mean; q += d * d; }
+  row_sum<16>(q, zero, box, wave);
+  const float rstd = 1.0f / sqrtf(q / (float)a.C + a.eps);
+  T* y = static_cast<T*>(a.y) + row * a.y_row;
+  for (int c = threadIdx.x; c < a.C; c += 1024) {
+    float o = ((float)x[c] - mean) * rstd, w;
+    if (a.w) { load_w<T, 1>(a.w, a.w32, c, &w); o *= w; }
+    if (a.b) { load_w<T, 1>(a.b, a.w32, c, &w); o += w; }
+    y[c] = (T)o;
+  }
+  if (threadIdx.x == 0 && a.mean) { a.mean[row] = mean; a.rstd[row] = rstd; }
+}
+template <class T>
+__global__ __launch_bounds__(1024) void norm_backward_wide_kernel(const NormArgs a) {
+  __shared__ float box[16][2];
+  const int wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_row;
+  const T* dy = static_cast<const T*>(a.dy) + row * a.dy_row;
+  const float mean = a.mean_in[row], rstd = a.rstd_in[row];
+  float s1 = 0.f, s2 = 0.f;
+  for (int c = threadIdx.x; c < a.C; c += 1024) {
+    float w = 1.f;
+    if (a.w) load_w<T, 1>(a.w, a.w32, c, &w);
+    const float g = (float)dy[c] * w;
+    s1 += g;
+    s2 += g * (((float)x[c] - mean) * rstd);
+  }
+  row_sum<16>(s1, s2, box, wave);
+  s1 /= (float)a.C;
+  s2 /= (float)a.C;
+  T* dx = static_cast<T*>(a.dx) + row * a.dx_row;
+  for (int c = threadIdx.x; c < a.C; c += 1024) {
+    float w = 1.f;
+    if (a.w) load_w<T, 1>(a.w, a.w32, c, &w);
+    dx[c] = (T)(rstd * ((float)dy[c] * w - s1 - ((float)x[c] - mean) * rstd * s2));
+  }
+}
+// ... and their columns: thread -> column, block row -> its share of the rows
+template <class T>
+__global__ __launch_bounds__(256) void norm_columns_kernel(const NormArgs a) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.C) return;
+  float dw = 0.f, db = 0.f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const float g = (float)(static_cast<const T*>(a.dy) + row * a.dy_row)[c];
+    dw += g * (((float)(static_cast<const T*>(a.x) + row * a.x_row)[c] - a.mean_in[row]) * a.rstd_in[row]);
+    db += g;
+  }
+  a.part[(size_t)blockIdx.y * 2 * a.C + c] = dw;
+  a.part[(size_t)blockIdx.y * 2 * a.C + a.C + c] = db;
+}
+
+// Adds the blocks' shares: 32 columns x 8 groups of blocks per block
+template <class T>
+__global__ __launch_bounds__(256) void norm_join_kernel(const NormArgs a) {
+  __shared__ float sums[8][33];
+  const int col = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + col;             // over 2 C: dw, then db
+  float s = 0.f;
+  if (c < 2 * a.C)
+    for (int b = grp; b < a.blocks; b += 8) s += a.part[(size_t)b * 2 * a.C + c];
+  sums[grp][col] = s;
+  __syncthreads();
+  if (grp || c >= 2 * a.C) return;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += sums[i][col];
+  void* out = c < a.C ? a.dw : a.db;
+  const int at = c < a.C ? c : c - a.C;
+  if (!out) return;
+  if (a.w32) static_cast<float*>(out)[at] = s;
+  else static_cast<T*>(out)[at] = (T)s;
+}
+
+// ---- which instance takes a width: VEC entries per access, N accesses per thread, W waves per row; N = 0: the wide kernels
+struct Choice { int vec, n, w; };
+Choice choose(int C, int size, bool aligned) {
+  Choice k;
+  k.vec = aligned ? 16 / size : 1;
+  const int64_t chunks = ((int64_t)C + k.vec - 1) / k.vec;
+  const int most = aligned ? 16 / k.vec : 16;       // 16 entries of a row per thread
+  for (int w : {1, 4, 16}) {
+    k.w = w;
+    for (int n = 1; n <= most; n *= 2) {
+      k.n = n;
+      if (chunks <= (int64_t)64 * w * n) return k;
+    }
+  }
+  k.n = 0;
+  return k;
+}
+int backward_blocks(int64_t rows, int C, const Choice& k) {    // blocks of the row walk (their shares are 8 C bytes each)
+  const int per = k.n == 0 ? 1 : k.w >= 4 ? 1 : 4 / k.w;
+  const int64_t most = k.w == 16 ? 256 : 1024;
+  return (int)max((int64_t)1, min((rows + per - 1) / per, k.n == 0 ? min((int64_t)64, rows) : most / per));
+}
+
+template <class T, int VEC, int N, int W>
+void launch_one(const NormArgs& a, bool backward, hipStream_t s) {
+  constexpr int R = W >= 4 ? 1 : 4 / W, threads = W > 4 ? 64 * W : 256;
+  if (backward) hipLaunchKernelGGL((norm_backward_kernel<T, VEC, N, W>), dim3(a.blocks / R), dim3(threads), 0, s, a);
+  else hipLaunchKernelGGL((norm_forward_kernel<T, VEC, N, W>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(threads), 0, s, a);
+}
+template <class T, int VEC, int N>
+void launch_w(const NormArgs& a, int w, bool backward, hipStream_t s) {
+  if (w == 1) launch_one<T, VEC, N, 1>(a, backward, s);
+  else if (w == 4) launch_one<T, VEC, N, 4>(a, backward, s);
+  else launch_one<T, VEC, N, 16>(a, backward, s);
+}
+template <class T, int VEC>
+void launch_n(const NormArgs& a, int n, int w, bool backward, hipStream_t s) {
+  constexpr int most = 16 / VEC;
+  if (n == 1) return launch_w<T, VEC, 1>(a, w, backward, s);
+  if constexpr (most >= 2) { if (n == 2) return launch_w<T, VEC, 2>(a, w, backward, s); }
+  if constexpr (most >= 4) { if (n == 4) return launch_w<T, VEC, 4>(a, w, backward, s); }
+  if constexpr (most >= 8) { if (n == 8) return launch_w<T, VEC, 8>(a, w, backward, s); }
+  if constexpr (most >= 16) { if (n == 16) return launch_w<T, VEC, 16>(a, w, backward, s); }
+}
+template <class T>
+void launch(const NormArgs& a, const Choice& k, bool backward, hipStream_t s) {
+  if (k.n == 0) {
+    if (!backward) hipLaunchKernelGGL((norm_forward_wide_kernel<T>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);
+    else {
+      if (a.dx) hipLaunchKernelGGL((norm_backward_wide_kernel<T>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);
+      if (a.part) hipLaunchKernelGGL((norm_columns_kernel<T>), dim3((a.C + 255) / 256, a.blocks), dim3(256), 0, s, a);
+    }
+  } else if (k.vec == 1) launch_n<T, 1>(a, k.n, k.w, backward, s);
+  else launch_n<T, 16 / (int)sizeof(T)>(a, k.n, k.w, backward, s);
+  if (backward && a.part) hipLaunchKernelGGL((norm_join_kernel<T>), dim3((2 * a.C + 31) / 32), dim3(256), 0, s, a);
+}
+
+int check(const ac_norm_args* p, const char* what) {
+  AC_REQUIRE(p, "%s: null arguments", what);
+  AC_REQUIRE(p->type == AC_F32 || p->type == AC_F16 || p->type == AC_BF16, "%s: unknown type %d", what, p->type);
+  AC_REQUIRE(p->weight_type == p->type || p->weight_type == AC_F32, "%s: weights must be fp32 or of the rows' type", what);
+  AC_REQUIRE(p->rows >= 0 && p->rows < (1LL << 31), "%s: bad number of rows", what);
+  AC_REQUIRE(p->width >= 1 && p->width <= 1 << 20, "%s: width %d must be in 1 .. 2^20", what, p->width);
+  return AC_OK;
+}
+// 16-byte accesses where every address allows them
+bool aligned16(const ac_norm_args* p, std::initializer_list<const void*> rows_of, std::initializer_list<int64_t> strides) {
+  const int size = p->type == AC_F32 ? 4 : 2, vec = 16 / size;
+  if (p->width % vec) return false;
+  for (const void* q : rows_of) if ((uintptr_t)q & 15) return false;
+  for (int64_t s : strides) if (s % vec) return false;
+  return ((uintptr_t)p->weight & 15) == 0 && ((uintptr_t)p->bias & 15) == 0;
+}
+
+}  // namespace
+
+extern "C" int ac_layer_norm(const ac_norm_args* p, void* stream) {
+  if (int rc = check(p, "ac_layer_norm")) return rc;
+  if (p->rows == 0) return AC_OK;
+  AC_REQUIRE(p->x && p->y, "ac_layer_norm: null pointer");
+  AC_REQUIRE(!p->mean == !p->rstd, "ac_layer_norm: mean and rstd come together");
+  const int size = p->type == AC_F32 ? 4 : 2, wsize = p->weight_type == AC_F32 ? 4 : 2;
+  AC_REQUIRE(((uintptr_t)p->x | (uintptr_t)p->y) % size == 0 && ((uintptr_t)p->weight | (uintptr_t)p->bias) % wsize == 0 &&
+             (((uintptr_t)p->mean | (uintptr_t)p->rstd) & 3) == 0, "ac_layer_norm: misaligned pointer");
+  NormArgs a = {};
+  a.x = p->x; a.y = p->y; a.w = p->weight; a.b = p->bias; a.x_row = p->x_row; a.y_row = p->y_row;
+  a.mean = p->mean; a.rstd = p->rstd; a.rows = p->rows; a.C = p->width; a.w32 = p->weight_type == AC_F32; a.eps = p->eps;
+  const Choice k = choose(p->width, size, aligned16(p, {p->x, p->y}, {p->x_row, p->y_row}));
+  if (p->type == AC_F32) launch<float>(a, k, false, as_stream(stream));
+  else if (p->type == AC_F16) launch<_Float16>(a, k, false, as_stream(stream));
+  else launch<__bf16>(a, k, false, as_stream(stream));
+  return ac_check_launch("ac_layer_norm");
+}
+
+// (the number of shares does not go by alignment: a workspace for the scalar kernels serves the others)
+static int norm_shares(const ac_norm_args* p, bool aligned) {
+  const Choice k = choose(p->width, p->type == AC_F32 ? 4 : 2, aligned);
+  const int per = k.n == 0 ? 1 : k.w >= 4 ? 1 : 4 / k.w;
+  return backward_blocks(p->rows, p->width, k) * per;
+}
+
+extern "C" size_t ac_layer_norm_backward_workspace_bytes(const ac_norm_args* p) {
+  if (check(p, "ac_layer_norm_backward") != AC_OK || p->rows == 0 || (!p->dweight && !p->dbias)) return 0;
+  return (size_t)max(norm_shares(p, true), norm_shares(p, false)) * 2 * p->width * sizeof(float);
+}
+
+extern "C" int ac_layer_norm_backward(const ac_norm_args* p, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check(p, "ac_layer_norm_backward")) return rc;
+  const int size = p->type == AC_F32 ? 4 : 2, wsize = p->weight_type == AC_F32 ? 4 : 2;
+  AC_REQUIRE(((uintptr_t)p->x | (uintptr_t)p->dy | (uintptr_t)p->dx) % size == 0 && (((uintptr_t)p->mean | (uintptr_t)p->rstd) & 3) == 0 &&
+             ((uintptr_t)p->weight | (uintptr_t)p->dweight | (uintptr_t)p->dbias) % wsize == 0, "ac_layer_norm_backward: misaligned pointer");
+  AC_REQUIRE(p->rows == 0 || (p->x && p->dy && p->mean && p->rstd), "ac_layer_norm_backward: null pointer");
+  NormArgs a = {};
+  a.x = p->x; a.dy = p->dy; a.dx = p->dx; a.w = p->weight; a.x_row = p->x_row; a.dy_row = p->dy_row; a.dx_row = p->dx_row;
+  a.mean_in = p->mean; a.rstd_in = p->rstd; a.dw = p->dweight; a.db = p->dbias;
+  a.rows = p->rows; a.C = p->width; a.w32 = p->weight_type == AC_F32;
+  const size_t need = ac_layer_norm_backward_workspace_bytes(p);
+  if (need && (!ws || ws_bytes < need)) return ac_fail(AC_EWORKSPACE, "ac_layer_norm_backward: workspace %zu < %zu", ws ? ws_bytes : (size_t)0, need);
+  AC_REQUIRE(((uintptr_t)ws & 3) == 0, "ac_layer_norm_backward: misaligned workspace");
+  if (!p->dx && !p->dweight && !p->dbias) return AC_OK;
+  const bool al = aligned16(p, {p->x, p->dy, p->dx}, {p->x_row, p->dy_row, p->dx_row});
+  const Choice k = choose(p->width, size, al);
+  a.blocks = norm_shares(p, al);
+  a.part = need ? static_cast<float*>(ws) : nullptr;
+  if (p->rows == 0) {                              // nothing to walk over: the sums are zero
+    a.blocks = 0;
+    if (p->dweight || p->dbias) {
+      if (p->type == AC_F32) hipLaunchKernelGGL((norm_join_kernel<float>), dim3((2 * a.C + 31) / 32), dim3(256), 0, as_stream(stream), a);
+      else if (p->type == AC_F16) hipLaunchKernelGGL((norm_join_kernel<_Float16>), dim3((2 * a.C + 31) / 32), dim3(256), 0, as_stream(stream), a);
+      else hipLaunchKernelGGL((norm_join_kernel<__bf16>), dim3((2 * a.C + 31) / 32), dim3(256), 0, as_stream(stream), a);
+    }
+    return ac_check_launch("ac_layer_norm_backward");
+  }
+  if (p->type == AC_F32) launch<float>(a, k, true, as_stream(stream));
+  else if (p->type == AC_F16) launch<_Float16>(a, k, true, as_stream(stream));
+  else launch<__bf16>(a, k, true, as_stream(stream));
+  return ac_check_launch("ac_layer_norm_backward");
+}

@@ -48,6 +48,13 @@ class AttentionArgs(_c.Structure):
                 + [(n, _i) for n in ("sequences", "heads", "kv_heads", "dim", "max_q", "max_k", "causal", "clear", "type")] + [("scale", _f)])
 
 
+class NormArgs(_c.Structure):
+    """struct ac_norm_args (include/ac_hip.h)."""
+    _fields_ = ([(n, _vp) for n in ("x", "weight", "bias", "y", "dy", "dx", "dweight", "dbias", "mean", "rstd")]
+                + [(n, _i64) for n in ("x_row", "y_row", "dy_row", "dx_row", "rows")]
+                + [(n, _i) for n in ("width", "type", "weight_type")] + [("eps", _f)])
+
+
 ABI_VERSION = 600      # include/ac_hip.h AC_ABI_VERSION
 
 # name -> (restype, argtypes): every symbol include/ac_hip.h declares
@@ -99,6 +106,9 @@ SIGNATURES = {
     "ac_rotary": (_i, [_c.POINTER(RotaryArgs), _vp]),
     "ac_attention_packed_workspace_bytes": (_sz, [_c.POINTER(AttentionArgs)]),
     "ac_attention_packed": (_i, [_c.POINTER(AttentionArgs), _vp, _sz, _vp]),
+    "ac_layer_norm": (_i, [_c.POINTER(NormArgs), _vp]),
+    "ac_layer_norm_backward_workspace_bytes": (_sz, [_c.POINTER(NormArgs)]),
+    "ac_layer_norm_backward": (_i, [_c.POINTER(NormArgs), _vp, _sz, _vp]),
     "ac_cluster_scores": (_i, [_vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp]),
 }
 
@@ -1077,3 +1087,98 @@ def _aligned(t):
     """Every head starts at a multiple of 16 bytes, as the kernels load them."""
     size = t.element_size()
     return t.data_ptr() % 16 == 0 and all(n <= 1 or s * size % 16 == 0 for n, s in zip(t.shape[:2], t.stride()[:2]))
+
+
+def _rows(t, name, like=None):
+    """`t` [..., width] as [rows, width] with neighbouring entries (a copy only where its axes do not fold into one stride)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError("%s must be a tensor on the HIP device (got %s); the MI355X path has no CPU fallback"
+                           % (name, getattr(t, "device", type(t))))
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError("%s must be [..., width], got %s" % (name, tuple(t.shape)))
+    if t.dtype not in _TYPES:
+        raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise RuntimeError("%s requires a gradient: this operator records no graph (layer_norm_backward has the gradients)" % name)
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError("%s is %s %s on %s, but x is %s %s on %s" % (name, t.dtype, tuple(t.shape), t.device, like.dtype, tuple(like.shape), like.device))
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _norm_vector(t, name, x):
+    if not isinstance(t, torch.Tensor) or t.device != x.device:
+        raise RuntimeError("%s must be a tensor on %s (got %s)" % (name, x.device, getattr(t, "device", type(t))))
+    if tuple(t.shape) != (x.shape[-1],):
+        raise ValueError("%s must be [%d], got %s" % (name, x.shape[-1], tuple(t.shape)))
+    if t.dtype not in (x.dtype, torch.float32):
+        raise TypeError("%s must be %s or float32, got %s" % (name, x.dtype, t.dtype))
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise RuntimeError("%s requires a gradient: this operator records no graph (layer_norm_backward has the gradients)" % name)
+    return t.contiguous()
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, want_stats=False):
+    """Layer norm over the last axis of x [..., width] (include/ac_hip.h ac_layer_norm): float32, float16 or bfloat16 of any width;
+    weight and bias [width] in x's type or float32 (both the same), or None.  out: where to write (x itself is allowed).
+    want_stats: also the fp32 mean and 1 / standard deviation of each row, which layer_norm_backward takes."""
+    rows = _rows(x, "x")
+    weight = None if weight is None else _norm_vector(weight, "weight", x)
+    bias = None if bias is None else _norm_vector(bias, "bias", x)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError("weight is %s, but bias is %s" % (weight.dtype, bias.dtype))
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    to = _rows(out, "out", x)
+    if to.data_ptr() != out.data_ptr():
+        raise ValueError("out: its axes must fold into rows of one stride, entries neighbours (strides %s)" % (tuple(out.stride()),))
+    _writable(out, "out")
+    for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
+        if t is not None and not _disjoint(out, t) and not (t is x and _same_view(out, x)):
+            raise ValueError("out overlaps %s" % name)
+    a = NormArgs()
+    a.x, a.y, a.x_row, a.y_row = rows.data_ptr(), to.data_ptr(), _row_stride(rows), _row_stride(to)
+    a.weight, a.bias = None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr()
+    a.rows, a.width, a.type, a.eps = rows.shape[0], rows.shape[1], _TYPES[x.dtype], float(eps)
+    a.weight_type = _TYPES[next((t.dtype for t in (weight, bias) if t is not None), torch.float32)]
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
+        a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
+    with torch.cuda.device(x.device):
+        _check(lib().ac_layer_norm(_c.byref(a), _stream()))
+    return (out, mean, rstd) if want_stats else out
+
+
+def layer_norm_backward(dy, x, weight, mean, rstd, want=(True, True, True)):
+    """Gradients of layer_norm at x: (dx, dweight, dbias), in x's and the weight's type (float32 without a weight); mean and rstd as
+    layer_norm(want_stats=True) returned them.  want: which of the three to compute (None in place of the others)."""
+    rows, grads = _rows(x, "x"), _rows(dy, "dy", x)
+    weight = None if weight is None else _norm_vector(weight, "weight", x)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        _whole(t, (torch.float32,), name, x.device)
+        if t.shape != x.shape[:-1]:
+            raise ValueError("%s must be %s, got %s" % (name, tuple(x.shape[:-1]), tuple(t.shape)))
+    kind = torch.float32 if weight is None else weight.dtype
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want[0] else None
+    dw, db = (torch.empty(rows.shape[1], dtype=kind, device=x.device) if w else None for w in want[1:])
+    a = NormArgs()
+    a.x, a.dy, a.x_row, a.dy_row, a.dx_row = rows.data_ptr(), grads.data_ptr(), _row_stride(rows), _row_stride(grads), rows.shape[1]
+    a.weight, a.mean, a.rstd = None if weight is None else weight.data_ptr(), mean.data_ptr(), rstd.data_ptr()
+    for name, t in (("dx", dx), ("dweight", dw), ("dbias", db)):
+        setattr(a, name, None if t is None else t.data_ptr())
+    a.rows, a.width, a.type, a.weight_type = rows.shape[0], rows.shape[1], _TYPES[x.dtype], _TYPES[kind]
+    with torch.cuda.device(x.device):
+        n = lib().ac_layer_norm_backward_workspace_bytes(_c.byref(a))
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None       # of this call alone, as in attention_packed
+        _check(lib().ac_layer_norm_backward(_c.byref(a), ws.data_ptr() if n else None, n, _stream()))
+    return dx, dw, db
+
+
+def _disjoint(a, b):
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a1 <= b0 or b1 <= a0

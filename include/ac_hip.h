@@ -374,6 +374,23 @@ typedef struct ac_attention_args {
 size_t ac_attention_packed_workspace_bytes(const ac_attention_args* args);
 int ac_attention_packed(const ac_attention_args* args, void* ws, size_t ws_bytes, void* stream);
 
+/* Layer norm of rows of any width (1 .. 2^20) and row stride, in fp32, fp16 or bf16 with weights of the same type or fp32:
+ * y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(variance + eps), statistics in fp32; weight and bias may be null.  mean, rstd
+ * (both or neither): fp32 [rows], what the backward pass takes.  y may be x with the same stride.
+ * ac_layernorm_rows above is the fp32 form that the ViT's final norm uses. */
+typedef struct ac_norm_args {
+  const void *x, *weight, *bias; void* y;
+  const void* dy; void *dx, *dweight, *dbias;      /* backward only */
+  float *mean, *rstd;
+  int64_t x_row, y_row, dy_row, dx_row, rows;
+  int32_t width, type, weight_type;
+  float eps;
+} ac_norm_args;
+int ac_layer_norm(const ac_norm_args* args, void* stream);
+/* Its gradients: dx (rows), dweight and dbias (summed over the rows in fp32 in a fixed order); null ones are not computed. */
+size_t ac_layer_norm_backward_workspace_bytes(const ac_norm_args* args);
+int ac_layer_norm_backward(const ac_norm_args* args, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

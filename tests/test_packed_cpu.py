@@ -118,3 +118,39 @@ def test_oracle_against_itself():
     assert torch.allclose(r["out"], torch.einsum("hij,jhd->ihd", p, v))
     r = opacked.attention(q, k[:2], v[:2], [0, 6], [0, 2], True)
     assert (r["out"][:4] == 0).all() and (r["sums"][:4] == -math.inf).all() and torch.allclose(r["out"][4], v[0])
+
+
+def _norm(**over):
+    a = acnative.NormArgs()
+    a.x = a.y = a.dy = a.dx = a.weight = a.bias = 4096
+    a.mean = a.rstd = 4096
+    a.x_row = a.y_row = a.dy_row = a.dx_row = 64
+    a.rows, a.width, a.type, a.weight_type, a.eps = 4, 64, 2, 0, 1e-6
+    for k, v in over.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("over,text", [({"type": 7}, "unknown type"), ({"weight_type": 1}, "weights"), ({"rows": -1}, "rows"), ({"rows": 1 << 31}, "rows"),
+                                       ({"width": 0}, "width"), ({"width": (1 << 20) + 1}, "width"), ({"x": 0}, "null"), ({"y": 0}, "null"),
+                                       ({"mean": 0}, "together"), ({"x": 4097}, "misaligned"), ({"weight": 4098}, "misaligned")])
+def test_layer_norm_refuses(over, text):
+    lib = acnative.lib()
+    assert lib.ac_layer_norm(ctypes.byref(_norm(**over)), None) == 1
+    assert text in lib.ac_last_error().decode()
+
+
+def test_layer_norm_backward_refuses_and_asks_for_its_workspace():
+    lib = acnative.lib()
+    for over, text in (({"dy": 0}, "null"), ({"mean": 0}, "null"), ({"dx": 4097}, "misaligned"), ({"dweight": 4098}, "misaligned"), ({"width": 0}, "width")):
+        assert lib.ac_layer_norm_backward(ctypes.byref(_norm(**over)), None, 0, None) == 1
+        assert text in lib.ac_last_error().decode()
+    n = lib.ac_layer_norm_backward_workspace_bytes(ctypes.byref(_norm(dweight=4096)))
+    assert n >= 2 * 64 * 4 and lib.ac_layer_norm_backward_workspace_bytes(ctypes.byref(_norm())) == 0
+    assert lib.ac_layer_norm_backward(ctypes.byref(_norm(dweight=4096)), 4096, n - 1, None) == 2 and b"workspace" in lib.ac_last_error()
+    assert lib.ac_layer_norm_backward(ctypes.byref(_norm(dx=0)), None, 0, None) == 0      # nothing wanted
+    assert lib.ac_layer_norm(ctypes.byref(_norm(rows=0)), None) == 0
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        acnative.layer_norm(torch.zeros(4, 8))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        acnative.layer_norm_backward(torch.zeros(4, 8), torch.zeros(4, 8), None, torch.zeros(4), torch.zeros(4))
