@@ -101,12 +101,67 @@ struct Shape {
   static constexpr int BUF = 2 * TILE;
   static constexpr int JOIN = WK > 1 ? (WK - 1) * WQ * NQ * 64 * (DB * 16 + 2) * 4 : 0;
   static constexpr int LDS = (2 * BUF + 256 > JOIN ? 2 * BUF + 256 : JOIN);
+  static constexpr int REGS = NQ * (NS * 4 + DB * 16 + 16 + (sizeof(T) == 2 ? 8 : 0)) + 48;   // queries, output, scores, weights; the rest
+  static constexpr int WAVES = REGS <= 128 && LDS <= 40960 ? 4 : REGS <= 168 && LDS <= 54000 ? 3 : REGS <= 256 && LDS <= 81920 ? 2 : 1;
   static constexpr int NI = TILE / 1024;                                   // transfers of 64 x 16 bytes per tile of K (or V)
   static constexpr int NJ = (NI + W - 1) / W;
 };
 
+// Rows [first, last) of a wave once more, key by key, over the keys that each sees alone: where values that some row does not see
+// are infinite or NaN.  Lane -> key for the scores, -> entries of the head for the sum.  Not made to be fast.
+template <class T, int DMAX>
+__device__ inline void again(const AttArgs& a, int split, int begin, int end, int q0, int nq, int k0, int nk, int kvh, int first, int last, int lane) {
+  constexpr int ND = (DMAX + 63) / 64;
+  for (int row = first; row < last; ++row) {
+    const int i = row / a.group, hh = kvh * a.group + row - i * a.group;
+    const int seen = min(end, a.causal ? min(max(i + nk - nq + 1, 0), nk) : nk);
+    const T* q = static_cast<const T*>(a.q) + (int64_t)(q0 + i) * a.q_tok + (int64_t)hh * a.q_head;
+    float m = NO_MAX, l = 0.f, o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = 0.f;
+    const float c = a.q_keep ? (a.q_flip ? -a.c_log2 : a.c_log2) : 0.f;
+    for (int key = begin; key < seen; key += 64) {
+      const int n = min(64, seen - key);
+      float s = -__builtin_inff();
+      if (lane < n) {
+        const T* k = static_cast<const T*>(a.k) + (int64_t)(k0 + key + lane) * a.k_tok + (int64_t)kvh * a.k_head;
+        float dot = 0.f;
+        for (int d = 0; d < a.dim; ++d) dot = __builtin_fmaf((float)q[d], (float)k[d], dot);
+        s = dot * c;
+      }
+      const float m_new = fmaxf(m, wave_max(s)), corr = __builtin_amdgcn_exp2f(m - m_new), p = __builtin_amdgcn_exp2f(s - m_new);
+      l = l * corr + wave_sum(p);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= corr;
+      for (int j = 0; j < n; ++j) {
+        const float w = __shfl(p, j, 64);
+        const T* v = static_cast<const T*>(a.v) + (int64_t)(k0 + key + j) * a.v_tok + (int64_t)kvh * a.v_head;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+          if (lane + 64 * d < a.dim) o[d] = __builtin_fmaf(w, (float)v[lane + 64 * d], o[d]);
+      }
+      m = m_new;
+    }
+    const size_t at = (size_t)(q0 + i) * a.heads + hh;
+    if (a.splits > 1) {
+      const size_t part = (size_t)split * a.tokens_q * a.heads + at;
+      if (lane == 0) { a.part_ml[2 * part] = m; a.part_ml[2 * part + 1] = l; }
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        if (lane + 64 * d < a.dim) a.part_o[part * a.dim + lane + 64 * d] = o[d];
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      T* out = static_cast<T*>(a.out) + (int64_t)(q0 + i) * a.o_tok + (int64_t)hh * a.o_head;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        if (lane + 64 * d < a.dim) out[lane + 64 * d] = (T)(o[d] * inv);
+      if (a.sums && lane == 0) a.sums[at] = l == 0.f ? -__builtin_inff() : 0.69314718055994530942f * (m + __builtin_amdgcn_logf(l));
+    }
+  }
+}
+
 template <class T, int NS, int NQ, int WQ, int WK, int KB>
-__global__ __launch_bounds__(64 * WQ * WK) void packed_attention_kernel(const AttArgs a) {
+__global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)) void packed_attention_kernel(const AttArgs a) {
   typedef Shape<T, NS, NQ, WQ, WK, KB> G;
   typedef Slots<NS> L;
   typedef Num<T> N;
@@ -187,7 +242,8 @@ __global__ __launch_bounds__(64 * WQ * WK) void packed_attention_kernel(const At
     const int block_last = min(tile_row + G::ROWS, rows) - 1;
     const int key_end = min(split_end, limit(block_last));
     const bool active = wave_row < rows;
-    const int lim_least = active ? limit(wave_row) : 0, lim_most = active ? limit(min(wave_row + 32 * NQ, rows) - 1) : 0;
+    bool odd_values = false;                       // an infinity or NaN among values that not every row of the wave sees
+    const int lim_least = active ? limit(wave_row) : 0, lim_most = active ? min(key_end, limit(min(wave_row + 32 * NQ, rows) - 1)) : 0;
     int lim[NQ];
     frag qf[NQ][NS];
 #pragma unroll
@@ -217,35 +273,47 @@ __global__ __launch_bounds__(64 * WQ * WK) void packed_attention_kernel(const At
         for (int i = 0; i < 16; ++i) o[b][d][i] = 0.f;
     }
 
-    // 32 keys, from LDS row `krow` of a tile on; key: the first one's number
-    auto block = [&](const uint8_t* Kt, const uint8_t* Vt, int krow, int key, auto masked_tag) {
-      constexpr bool MASKED = decltype(masked_tag)::value;
+    // 32 keys, from LDS row `krow` of a tile on; key: the first one's number.  masked (uniform): some row does not see them all
+    const int kturn = L::k_turn(r);
+    const int vq = (lane & 15) >> 2, vp = lane & 3, vg = (lane >> 4) & 1;
+    auto block = [&](const uint8_t* Kt, const uint8_t* Vt, int krow, int key, bool masked) {
       f32x16 sc[NQ];
 #pragma unroll
       for (int b = 0; b < NQ; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[b][i] = 0.f;
       const uint8_t* krp = Kt + (krow + r) * P;
-      const int kt = L::k_turn(r);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        const frag kf = *reinterpret_cast<const frag*>(krp + L::place(2 * s + h, kt) * 16);
+        const frag kf = *reinterpret_cast<const frag*>(krp + L::place(2 * s + h, kturn) * 16);
 #pragma unroll
         for (int b = 0; b < NQ; ++b) sc[b] = N::mfma(kf, qf[b][s], sc[b]);
       }
+      if (masked) {
 #pragma unroll
-      for (int b = 0; b < NQ; ++b) {
-        if constexpr (MASKED) {
+        for (int b = 0; b < NQ; ++b)
 #pragma unroll
           for (int i = 0; i < 16; ++i) sc[b][i] = key + 8 * (i >> 2) + 4 * h + (i & 3) < lim[b] ? sc[b][i] : -__builtin_inff();
+        // A masked score has p = 0, but 0 times an infinity or NaN is NaN: rows of a wave that meets one here are done again
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(Vt + krow * P + j * 1024 + lane * 16);
+          odd |= N::odd(w[0]) | N::odd(w[1]) | N::odd(w[2]) | N::odd(w[3]);
         }
+        if (__builtin_amdgcn_ballot_w64(odd)) odd_values = true;
+        asm volatile("" ::: "memory");                 // (keeps this a branch: as selects it would cost every tile)
+      }
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
         float top = sc[b][0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[b][i]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float m_new = fmaxf(m_run[b], top * a.c_log2);
-        if (__builtin_amdgcn_ballot_w64(m_new != m_run[b])) {
-          const float corr = __builtin_amdgcn_exp2f(m_run[b] - m_new);
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c_log2;
+        // The sums keep an older maximum until one is 2^8 ahead of it: weights up to 256 cost no digits (they are rounded
+        // relative to themselves) and o is rescaled a few times per row instead of in most tiles
+        if (__builtin_amdgcn_ballot_w64(top > m_run[b] + 8.0f)) {
+          const float m_new = fmaxf(m_run[b], top), corr = __builtin_amdgcn_exp2f(m_run[b] - m_new);
           l_run[b] *= corr;
 #pragma unroll
           for (int d = 0; d < DB; ++d)
@@ -261,97 +329,48 @@ __global__ __launch_bounds__(64 * WQ * WK) void packed_attention_kernel(const At
         }
         l_run[b] += sum;
       }
-      // O^T += V^T P^T.  only >= 0: that key alone, for the rows that see it (below)
-      auto values = [&](const int only) {
-        constexpr int KS = N::wide ? 16 : 2;
-        auto key_of = [&](int i) { return 8 * (i >> 2) + 4 * h + (i & 3); };
+      // O^T += V^T P^T
+      if constexpr (N::wide) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int row = krow + 8 * (i >> 2) + 4 * h + (i & 3);
+            const float vf = *reinterpret_cast<const float*>(Vt + row * P + L::place(8 * d + (r >> 2), L::template v_turn<true>(4 * h)) * 16 + (r & 3) * 4);
+#pragma unroll
+            for (int b = 0; b < NQ; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, sc[b][i], o[b][d], 0, 0, 0);
+          }
+      } else {
         frag pf[NQ][2];
-        if constexpr (!N::wide) {
 #pragma unroll
-          for (int b = 0; b < NQ; ++b)
+        for (int b = 0; b < NQ; ++b)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              u32x4 w;
+          for (int ks = 0; ks < 2; ++ks) {
+            u32x4 w;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int i = 8 * ks + 2 * j;
-                w[j] = only < 0 ? N::pack(sc[b][i], sc[b][i + 1]) : N::pack(key_of(i) == only ? sc[b][i] : 0.f, key_of(i + 1) == only ? sc[b][i + 1] : 0.f);
-              }
-              pf[b][ks] = __builtin_bit_cast(frag, w);
+            for (int j = 0; j < 4; ++j) w[j] = N::pack(sc[b][8 * ks + 2 * j], sc[b][8 * ks + 2 * j + 1]);
+            pf[b][ks] = __builtin_bit_cast(frag, w);
+          }
+        // transposed reads: lane 4 q + p of a 16-lane group addresses key row q, entries 4 p .. of the group's 16, and gets
+        // column (lane & 15) of the 4 x 16 block; the groups take (entries 0 .. 15, 16 .. 31) x (lane halves)
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            u32x4 w;
+#pragma unroll
+            for (int j2 = 0; j2 < 2; ++j2) {
+              const int row = krow + 16 * ks + 8 * j2 + 4 * h + vq;
+              const uint8_t* at = Vt + row * P + L::place(4 * d + 2 * vg + (vp >> 1), L::template v_turn<false>(4 * h + vq)) * 16 + 8 * (vp & 1);
+              const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at)));
+              w[2 * j2] = x[0];
+              w[2 * j2 + 1] = x[1];
             }
-        }
-        // 16-bit, transposed reads: lane 4 q + p of a 16-lane group addresses key row q, entries 4 p .. of the group's 16, and
-        // gets column (lane & 15) of the 4 x 16 block; the groups take (entries 0 .. 15, 16 .. 31) x (lane halves)
-        const int q = (lane & 15) >> 2, p = lane & 3, g1 = (lane >> 4) & 1;
+            const frag vf = __builtin_bit_cast(frag, w);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          f32x16 part[NQ];
-          if (only >= 0) {
-#pragma unroll
-            for (int b = 0; b < NQ; ++b)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) part[b][i] = 0.f;
+            for (int b = 0; b < NQ; ++b) o[b][d] = N::mfma(vf, pf[b][ks], o[b][d]);
           }
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (N::wide) {
-              const int row = krow + key_of(ks);
-              float vf = *reinterpret_cast<const float*>(Vt + row * P + L::place(8 * d + (r >> 2), L::template v_turn<true>(row)) * 16 + (r & 3) * 4);
-              if (only >= 0 && key_of(ks) != only) vf = 0.f;
-#pragma unroll
-              for (int b = 0; b < NQ; ++b) {
-                if (only < 0) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, sc[b][ks], o[b][d], 0, 0, 0);
-                else part[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, key_of(ks) == only ? sc[b][ks] : 0.f, part[b], 0, 0, 0);
-              }
-            } else {
-              u32x4 w;
-#pragma unroll
-              for (int j2 = 0; j2 < 2; ++j2) {
-                const int row = krow + 16 * ks + 8 * j2 + 4 * h + q;
-                const uint8_t* at = Vt + row * P + L::place(4 * d + 2 * g1 + (p >> 1), L::template v_turn<false>(4 * h + q)) * 16 + 8 * (p & 1);
-                const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at)));
-                w[2 * j2] = x[0];
-                w[2 * j2 + 1] = x[1];
-              }
-              if (only >= 0) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int i = 8 * ks + 2 * j;
-                  w[j] = key_of(i) == only ? w[j] & 0xffffu : key_of(i + 1) == only ? w[j] & 0xffff0000u : 0u;
-                }
-              }
-              const frag vf = __builtin_bit_cast(frag, w);
-#pragma unroll
-              for (int b = 0; b < NQ; ++b) {
-                if (only < 0) o[b][d] = N::mfma(vf, pf[b][ks], o[b][d]);
-                else part[b] = N::mfma(vf, pf[b][ks], part[b]);
-              }
-            }
-          }
-          if (only >= 0) {
-#pragma unroll
-            for (int b = 0; b < NQ; ++b)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[b][d][i] = key + only < lim[b] ? o[b][d][i] + part[b][i] : o[b][d][i];
-          }
-        }
-      };
-      if constexpr (MASKED) {
-        // A masked score has p = 0, but 0 times an infinity or NaN is NaN: where these 32 values hold one, the keys are taken
-        // one by one and added to the rows that see them alone.
-        bool odd = false;
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(Vt + krow * P + j * 1024 + lane * 16);
-          odd |= N::odd(w[0]) | N::odd(w[1]) | N::odd(w[2]) | N::odd(w[3]);
-        }
-        if (__builtin_amdgcn_ballot_w64(odd)) {
-#pragma unroll 1
-          for (int only = 0; only < 32; ++only) values(only);
-          return;
-        }
       }
-      values(-1);
     };
 
     if (key_end > split_begin) fetch(split_begin, 0);
@@ -362,12 +381,10 @@ __global__ __launch_bounds__(64 * WQ * WK) void packed_attention_kernel(const At
       if (key + G::KEYS < key_end) fetch(key + G::KEYS, buffer ^ 1);
       const uint8_t* Kt = lds + buffer * G::BUF;
       const uint8_t* Vt = Kt + G::TILE;
-#pragma unroll
+#pragma unroll 1
       for (int kb = 0; kb < KB; ++kb) {
         const int krow = (wk * KB + kb) * 32, at = key + krow;
-        if (at >= min(lim_most, key_end)) continue;
-        if (at + 32 <= lim_least && at + 32 <= key_end) block(Kt, Vt, krow, at, std::false_type{});
-        else block(Kt, Vt, krow, at, std::true_type{});
+        if (at < lim_most) block(Kt, Vt, krow, at, at + 32 > lim_least);
       }
       buffer ^= 1;
     }
@@ -408,7 +425,18 @@ __global__ __launch_bounds__(64 * WQ * WK) void packed_attention_kernel(const At
           }
       }
     }
-    if (wk == 0) {
+    if constexpr (WK > 1) {
+      __syncthreads();
+      int* const flag = reinterpret_cast<int*>(lds);
+      if (tid == 0) *flag = 0;
+      __syncthreads();
+      if (odd_values && lane == 0) *flag = 1;      // WQ is 1 here: the block's waves share the rows
+      __syncthreads();
+      odd_values = *flag != 0;
+    }
+    if (wk == 0 && odd_values) {
+      again<T, DB * 32>(a, split, split_begin, split_end, q0, nq, k0, nk, kvh, wave_row, min(wave_row + 32 * NQ, rows), lane);
+    } else if (wk == 0) {
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
         const int row = wave_row + 32 * b + r;
