@@ -19,8 +19,6 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) void* lptr_t;
-typedef __amdgpu_buffer_rsrc_t rsrc_t;
 
 struct AttArgs {
   const void *q, *k, *v; void* out; float* sums;
@@ -88,6 +86,27 @@ template <int NS> struct Slots {
   }
 };
 
+__device__ inline uint32_t first_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+
+// 16 bytes per lane from a buffer into LDS at `at` (uniform) + 16 * lane; an offset behind the descriptor's end writes zeros.  As
+// assembly because the compiler, which cannot tell the tiles apart, waits for every transfer in flight before it reads any of
+// them; the kernel's own waits order both.  It writes no register but M0 (one wait state between that and its use).
+__device__ inline void to_lds(u32x4 rsrc, uint32_t offset, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(first_lane(at)), "v"(offset), "s"(rsrc) : "memory", "m0");
+}
+template <int N> __device__ inline void wait_transfers() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ inline void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// the larger of the two lane halves' values, in both
+__device__ inline float halves_max(float x) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t lower = p[0], upper = p[1];       // (a bit cast of p[1] itself reads p[0])
+  return fmaxf(__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper));
+}
+
 constexpr float NO_MAX = -3.0e38f;     // of a row that has seen no key: finite, so that no difference of infinities arises
 
 // NS: steps of 32 bytes of a row (dim rounded up); NQ: blocks of 32 rows per wave; WQ x WK waves: over rows x over keys;
@@ -99,9 +118,12 @@ struct Shape {
   static constexpr int E = 16 / (int)sizeof(T);                            // entries of a slot
   static constexpr int DB = (NS * 2 * E + 31) / 32;                        // blocks of 32 entries of the output
   static constexpr int BUF = 2 * TILE;
+  static constexpr bool RING = WQ > 1 && 4 * BUF + 256 <= 160 * 1024;  // the pipelined loop: four tiles; else two
+  static constexpr int BUFS = RING ? 4 : 2;
   static constexpr int JOIN = WK > 1 ? (WK - 1) * WQ * NQ * 64 * (DB * 16 + 2) * 4 : 0;
-  static constexpr int LDS = (2 * BUF + 256 > JOIN ? 2 * BUF + 256 : JOIN);
-  static constexpr int REGS = NQ * (NS * 4 + DB * 16 + 16 + (sizeof(T) == 2 ? 8 : 0)) + 48;   // queries, output, scores, weights; the rest
+  static constexpr int LDS = (BUFS * BUF + 256 > JOIN ? BUFS * BUF + 256 : JOIN);
+  // registers: queries, output, two blocks of scores, weights, K and V fragments, the rest
+  static constexpr int REGS = NQ * (NS * 4 + DB * 16 + (RING ? 32 : 16) + (sizeof(T) == 2 ? 8 : 0)) + (RING ? 2 * NS * 4 : 16) + 40;
   static constexpr int WAVES = REGS <= 128 && LDS <= 40960 ? 4 : REGS <= 168 && LDS <= 54000 ? 3 : REGS <= 256 && LDS <= 81920 ? 2 : 1;
   static constexpr int NI = TILE / 1024;                                   // transfers of 64 x 16 bytes per tile of K (or V)
   static constexpr int NJ = (NI + W - 1) / W;
@@ -214,20 +236,21 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
   }
   const uint8_t* const kbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.k) + (int64_t)k0 * a.k_tok + kvh * a.k_head);
   const uint8_t* const vbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.v) + (int64_t)k0 * a.v_tok + kvh * a.v_head);
+  const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   // tile of keys `key` .. : rows behind the sequence read as zero (the descriptor ends with its last entry)
   auto fetch = [&](int key, int buffer) {
     const int left = min(nk - key, G::KEYS);
     const uint64_t kb = (uint64_t)kbase + (uint64_t)key * ks_bytes, vb = (uint64_t)vbase + (uint64_t)key * vs_bytes;
     const uint32_t kn = (uint32_t)(left - 1) * ks_bytes + a.dim * sizeof(T), vn = (uint32_t)(left - 1) * vs_bytes + a.dim * sizeof(T);
-    const rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(kb), 0, kn, 0x00020000);
-    const rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(vb), 0, vn, 0x00020000);
-    uint8_t* const dst = lds + buffer * G::BUF;
+    const u32x4 kr = {first_lane((uint32_t)kb), first_lane((uint32_t)(kb >> 32)), first_lane(kn), 0x00020000u};
+    const u32x4 vr = {first_lane((uint32_t)vb), first_lane((uint32_t)(vb >> 32)), first_lane(vn), 0x00020000u};
+    const uint32_t dst = lds_base + buffer * G::BUF;
 #pragma unroll
     for (int j = 0; j < G::NJ; ++j) {
       const int n = wave + G::W * j;
       if (G::NI % G::W == 0 || n < G::NI) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lptr_t)(dst + n * 1024), 16, (int)koff[j], 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lptr_t)(dst + G::TILE + n * 1024), 16, (int)voff[j], 0, 0, 0);
+        to_lds(kr, koff[j], dst + n * 1024);
+        to_lds(vr, voff[j], dst + G::TILE + n * 1024);
       }
     }
   };
@@ -273,47 +296,55 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
         for (int i = 0; i < 16; ++i) o[b][d][i] = 0.f;
     }
 
-    // 32 keys, from LDS row `krow` of a tile on; key: the first one's number.  masked (uniform): some row does not see them all
     const int kturn = L::k_turn(r);
     const int vq = (lane & 15) >> 2, vp = lane & 3, vg = (lane >> 4) & 1;
-    auto block = [&](const uint8_t* Kt, const uint8_t* Vt, int krow, int key, bool masked) {
-      f32x16 sc[NQ];
+    // S^T of 32 keys, from LDS row `krow` of a tile on
+    auto scores = [&](const uint8_t* Kt, int krow, f32x16 (&sc)[NQ]) {
+      const uint8_t* krp = Kt + (krow + r) * P;
+      frag kf[NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) kf[s] = *reinterpret_cast<const frag*>(krp + L::place(2 * s + h, kturn) * 16);
 #pragma unroll
       for (int b = 0; b < NQ; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[b][i] = 0.f;
-      const uint8_t* krp = Kt + (krow + r) * P;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const frag kf = *reinterpret_cast<const frag*>(krp + L::place(2 * s + h, kturn) * 16);
+      for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int b = 0; b < NQ; ++b) sc[b] = N::mfma(kf, qf[b][s], sc[b]);
+        for (int b = 0; b < NQ; ++b) sc[b] = N::mfma(kf[s], qf[b][s], sc[b]);
+    };
+    // key: the block's first; some row of the wave does not see all of its keys
+    auto mask = [&](const uint8_t* Vt, int krow, int key, f32x16 (&sc)[NQ]) {
+#pragma unroll
+      for (int b = 0; b < NQ; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[b][i] = key + 8 * (i >> 2) + 4 * h + (i & 3) < lim[b] ? sc[b][i] : -__builtin_inff();
+      // A masked score has p = 0, but 0 times an infinity or NaN is NaN: rows of a wave that meets one here are done again
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(Vt + krow * P + j * 1024 + lane * 16);
+        odd |= N::odd(w[0]) | N::odd(w[1]) | N::odd(w[2]) | N::odd(w[3]);
       }
-      if (masked) {
-#pragma unroll
-        for (int b = 0; b < NQ; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[b][i] = key + 8 * (i >> 2) + 4 * h + (i & 3) < lim[b] ? sc[b][i] : -__builtin_inff();
-        // A masked score has p = 0, but 0 times an infinity or NaN is NaN: rows of a wave that meets one here are done again
-        bool odd = false;
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(Vt + krow * P + j * 1024 + lane * 16);
-          odd |= N::odd(w[0]) | N::odd(w[1]) | N::odd(w[2]) | N::odd(w[3]);
-        }
-        if (__builtin_amdgcn_ballot_w64(odd)) odd_values = true;
-        asm volatile("" ::: "memory");                 // (keeps this a branch: as selects it would cost every tile)
-      }
+      if (__builtin_amdgcn_ballot_w64(odd)) odd_values = true;
+      asm volatile("" ::: "memory");                   // (keeps this a branch: as selects it would cost every block)
+    };
+    auto maxima = [&](const f32x16 (&sc)[NQ], float (&top)[NQ]) {
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
-        float top = sc[b][0];
+        top[b] = sc[b][0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[b][i]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c_log2;
-        // The sums keep an older maximum until one is 2^8 ahead of it: weights up to 256 cost no digits (they are rounded
-        // relative to themselves) and o is rescaled a few times per row instead of in most tiles
-        if (__builtin_amdgcn_ballot_w64(top > m_run[b] + 8.0f)) {
-          const float m_new = fmaxf(m_run[b], top), corr = __builtin_amdgcn_exp2f(m_run[b] - m_new);
+        for (int i = 1; i < 16; ++i) top[b] = fmaxf(top[b], sc[b][i]);
+        top[b] = halves_max(top[b]) * a.c_log2;
+      }
+    };
+    // The sums keep an older maximum until one is 2^8 ahead of it: weights up to 256 cost no digits (they are rounded relative
+    // to themselves) and o is rescaled a few times per row instead of in most blocks
+    auto rescale = [&](const float (&top)[NQ]) {
+#pragma unroll
+      for (int b = 0; b < NQ; ++b)
+        if (__builtin_amdgcn_ballot_w64(top[b] > m_run[b] + 8.0f)) {
+          const float m_new = fmaxf(m_run[b], top[b]), corr = __builtin_amdgcn_exp2f(m_run[b] - m_new);
           l_run[b] *= corr;
 #pragma unroll
           for (int d = 0; d < DB; ++d)
@@ -321,6 +352,10 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
             for (int i = 0; i < 16; ++i) o[b][d][i] *= corr;
           m_run[b] = m_new;
         }
+    };
+    auto weights = [&](f32x16 (&sc)[NQ], frag (&pf)[NQ][2]) {
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -328,8 +363,21 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
           sum += sc[b][i];
         }
         l_run[b] += sum;
+        if constexpr (!N::wide) {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            u32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = N::pack(sc[b][8 * ks + 2 * j], sc[b][8 * ks + 2 * j + 1]);
+            asm volatile("" : "+v"(w));                // here, beside the products of the next scores, and not where it is used
+            pf[b][ks] = __builtin_bit_cast(frag, w);
+          }
+        }
       }
-      // O^T += V^T P^T
+    };
+    // O^T += V^T P^T.  16-bit, transposed reads: lane 4 q + p of a 16-lane group addresses key row q, entries 4 p .. of the group's
+    // 16, and gets column (lane & 15) of the 4 x 16 block; the groups take (entries 0 .. 15, 16 .. 31) x (lane halves)
+    auto values = [&](const uint8_t* Vt, int krow, const f32x16 (&sc)[NQ], const frag (&pf)[NQ][2]) {
       if constexpr (N::wide) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -341,18 +389,6 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
             for (int b = 0; b < NQ; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, sc[b][i], o[b][d], 0, 0, 0);
           }
       } else {
-        frag pf[NQ][2];
-#pragma unroll
-        for (int b = 0; b < NQ; ++b)
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            u32x4 w;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = N::pack(sc[b][8 * ks + 2 * j], sc[b][8 * ks + 2 * j + 1]);
-            pf[b][ks] = __builtin_bit_cast(frag, w);
-          }
-        // transposed reads: lane 4 q + p of a 16-lane group addresses key row q, entries 4 p .. of the group's 16, and gets
-        // column (lane & 15) of the 4 x 16 block; the groups take (entries 0 .. 15, 16 .. 31) x (lane halves)
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -373,20 +409,74 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
       }
     };
 
-    if (key_end > split_begin) fetch(split_begin, 0);
-    int buffer = 0;
-    for (int key = split_begin; key < key_end; key += G::KEYS) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (key + G::KEYS < key_end) fetch(key + G::KEYS, buffer ^ 1);
-      const uint8_t* Kt = lds + buffer * G::BUF;
-      const uint8_t* Vt = Kt + G::TILE;
-#pragma unroll 1
-      for (int kb = 0; kb < KB; ++kb) {
-        const int krow = (wk * KB + kb) * 32, at = key + krow;
-        if (at < lim_most) block(Kt, Vt, krow, at, at + 32 > lim_least);
+    const int tiles = key_end > split_begin ? (key_end - split_begin + G::KEYS - 1) / G::KEYS : 0;
+    if constexpr (G::RING) {
+      // Pipelined: block j's exponentials run beside the products of block j + 1's scores, its values beside their maxima.
+      // Tiles t + 1 and t + 2 are in flight while t is read; the buffer of t + 3 is the one of t - 1, which every wave has
+      // left when it passes the barrier in front of the last block of t.
+      constexpr int COUNT = 2 * (G::NI / G::W);        // transfers of a tile per wave (some waves issue two more: they wait longer)
+      const int blocks = (key_end - split_begin + 31) / 32, mine = (lim_most - split_begin + 31) / 32;
+#pragma unroll
+      for (int t = 0; t < 3; ++t)
+        if (t < tiles) fetch(split_begin + t * G::KEYS, t);
+      wait_transfers<0>();
+      barrier();
+      f32x16 sa[NQ], sb[NQ];
+      if (mine > 0) {
+        float top[NQ];
+        scores(lds, 0, sa);
+        if (split_begin + 32 > lim_least) mask(lds + G::TILE, 0, split_begin, sa);
+        maxima(sa, top);
+        rescale(top);
       }
-      buffer ^= 1;
+      auto step = [&](int j, f32x16 (&now)[NQ], f32x16 (&next)[NQ]) {
+        const int t = j / KB;
+        if (j % KB == KB - 1 && t + 1 < tiles) {       // the next block lies in the next tile
+          if (t + 2 < tiles) wait_transfers<COUNT>();
+          else wait_transfers<0>();
+          barrier();
+          if (t + 3 < tiles) fetch(split_begin + (t + 3) * G::KEYS, (t + 3) & 3);
+        }
+        if (j >= mine) return;
+        const uint8_t* Vt = lds + (t & 3) * G::BUF + G::TILE;
+        const int tn = (j + 1) / KB, krow = (j % KB) * 32, krow_n = ((j + 1) % KB) * 32, key_n = split_begin + (j + 1) * 32;
+        const uint8_t* Kn = lds + (tn & 3) * G::BUF;   // behind the last block: what is there, for nothing
+        frag pf[NQ][2];
+        float top[NQ];
+        scores(Kn, krow_n, next);
+        weights(now, pf);
+        const bool more = j + 1 < mine;
+        if (more && key_n + 32 > lim_least) mask(Kn + G::TILE, krow_n, key_n, next);
+        values(Vt, krow, now, pf);
+        maxima(next, top);
+        if (more) rescale(top);
+      };
+      for (int j = 0; j < blocks; j += 2) {
+        step(j, sa, sb);
+        if (j + 1 < blocks) step(j + 1, sb, sa);
+      }
+    } else {
+      if (tiles) fetch(split_begin, 0);
+      for (int t = 0; t < tiles; ++t) {
+        wait_transfers<0>();
+        barrier();
+        if (t + 1 < tiles) fetch(split_begin + (t + 1) * G::KEYS, (t + 1) & 1);
+        const uint8_t* Kt = lds + (t & 1) * G::BUF;
+#pragma unroll 1
+        for (int kb = 0; kb < KB; ++kb) {
+          const int krow = (wk * KB + kb) * 32, key = split_begin + t * G::KEYS + krow;
+          if (key >= lim_most) continue;
+          f32x16 sc[NQ];
+          frag pf[NQ][2];
+          float top[NQ];
+          scores(Kt, krow, sc);
+          if (key + 32 > lim_least) mask(Kt + G::TILE, krow, key, sc);
+          maxima(sc, top);
+          rescale(top);
+          weights(sc, pf);
+          values(Kt + G::TILE, krow, sc, pf);
+        }
+      }
     }
 
     // ---- the lane halves' sums, then the waves that took other keys

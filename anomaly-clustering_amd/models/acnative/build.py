@@ -21,6 +21,10 @@ FLAGS = ["-O3", "-std=c++17", "--offload-arch=" + ARCH, "-fPIC", "-ffp-contract=
          # scalar instructions compute the same bits (hipcc's host pass does not know the feature and says so: harmless)
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
+# attention.hip: matrix products accumulate in the vector registers that the softmax works on (the accumulation registers hold
+# the queries instead); otherwise every block of keys copies its output tile from one file to the other and back
+FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def _sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
@@ -58,7 +62,7 @@ def _build(force, verbose, LIB, OBJ_DIR, extra):
 
     def compile_one(src):
         obj = os.path.join(OBJ_DIR, os.path.basename(src)[:-4] + ".o")
-        cmd = [hipcc] + FLAGS + extra + ["-c", src, "-o", obj]
+        cmd = [hipcc] + FLAGS + FILE_FLAGS.get(os.path.basename(src), []) + extra + ["-c", src, "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("hipcc failed on %s:\n%s\n%s" % (src, r.stdout, r.stderr))
