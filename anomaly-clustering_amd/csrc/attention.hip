@@ -118,7 +118,7 @@ struct Shape {
   static constexpr int E = 16 / (int)sizeof(T);                            // entries of a slot
   static constexpr int DB = (NS * 2 * E + 31) / 32;                        // blocks of 32 entries of the output
   static constexpr int BUF = 2 * TILE;
-  static constexpr bool RING = WQ > 1 && 4 * BUF + 256 <= 160 * 1024;  // the pipelined loop: four tiles; else two
+  static constexpr bool RING = sizeof(T) == 2 && WQ > 1 && 4 * BUF + 256 <= 160 * 1024;  // the pipelined loop: four tiles; else two
   static constexpr int BUFS = RING ? 4 : 2;
   static constexpr int JOIN = WK > 1 ? (WK - 1) * WQ * NQ * 64 * (DB * 16 + 2) * 4 : 0;
   static constexpr int LDS = (BUFS * BUF + 256 > JOIN ? BUFS * BUF + 256 : JOIN);
@@ -281,6 +281,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
         u32x4 w = __builtin_bit_cast(u32x4, row < rows && d < a.dim ? *reinterpret_cast<const frag*>(src + d) : z);
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = (w[j] & a.q_keep) ^ a.q_flip;
+        if constexpr (G::WAVES == 1 && !N::wide) asm volatile("" : "+a"(w));       // in the accumulation registers, which the products read in place
         qf[b][s] = __builtin_bit_cast(frag, w);
       }
     }
@@ -356,13 +357,12 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
     auto weights = [&](f32x16 (&sc)[NQ], frag (&pf)[NQ][2]) {
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
-        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          sc[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], a.c_log2, -m_run[b]));
-          sum += sc[b][i];
-        }
-        l_run[b] += sum;
+        for (int i = 0; i < 16; ++i) sc[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], a.c_log2, -m_run[b]));
+        float part[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[i] = (sc[b][i] + sc[b][4 + i]) + (sc[b][8 + i] + sc[b][12 + i]);
+        l_run[b] += (part[0] + part[1]) + (part[2] + part[3]);
         if constexpr (!N::wide) {
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
@@ -375,12 +375,25 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
         }
       }
     };
-    // O^T += V^T P^T.  16-bit, transposed reads: lane 4 q + p of a 16-lane group addresses key row q, entries 4 p .. of the group's
-    // 16, and gets column (lane & 15) of the 4 x 16 block; the groups take (entries 0 .. 15, 16 .. 31) x (lane halves)
-    auto values = [&](const uint8_t* Vt, int krow, const f32x16 (&sc)[NQ], const frag (&pf)[NQ][2]) {
-      if constexpr (N::wide) {
+    // V^T fragments of 32 keys.  Transposed reads: lane 4 q + p of a 16-lane group addresses key row q, entries 4 p .. of the
+    // group's 16, and gets column (lane & 15) of the 4 x 16 block; the groups take (entries 0 .. 15, 16 .. 31) x (lane halves)
+    auto value_at = [&](const uint8_t* Vt, int krow, int d, int ks) {
+      u32x4 w;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+      for (int j2 = 0; j2 < 2; ++j2) {
+        const int row = krow + 16 * ks + 8 * j2 + 4 * h + vq;
+        const uint8_t* at = Vt + row * P + L::place(4 * d + 2 * vg + (vp >> 1), L::template v_turn<false>(4 * h + vq)) * 16 + 8 * (vp & 1);
+        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at)));
+        w[2 * j2] = x[0];
+        w[2 * j2 + 1] = x[1];
+      }
+      return w;
+    };
+    // O^T += V^T P^T
+    auto values = [&](const uint8_t* Vt, int krow, const f32x16 (&sc)[NQ], const frag (&pf)[NQ][2]) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        if constexpr (N::wide) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int row = krow + 8 * (i >> 2) + 4 * h + (i & 3);
@@ -388,24 +401,14 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
 #pragma unroll
             for (int b = 0; b < NQ; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, sc[b][i], o[b][d], 0, 0, 0);
           }
-      } else {
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
+        } else {
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
-            u32x4 w;
-#pragma unroll
-            for (int j2 = 0; j2 < 2; ++j2) {
-              const int row = krow + 16 * ks + 8 * j2 + 4 * h + vq;
-              const uint8_t* at = Vt + row * P + L::place(4 * d + 2 * vg + (vp >> 1), L::template v_turn<false>(4 * h + vq)) * 16 + 8 * (vp & 1);
-              const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at)));
-              w[2 * j2] = x[0];
-              w[2 * j2 + 1] = x[1];
-            }
-            const frag vf = __builtin_bit_cast(frag, w);
+            const frag vf = __builtin_bit_cast(frag, value_at(Vt, krow, d, ks));
 #pragma unroll
             for (int b = 0; b < NQ; ++b) o[b][d] = N::mfma(vf, pf[b][ks], o[b][d]);
           }
+        }
       }
     };
 
@@ -443,11 +446,28 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
         const uint8_t* Kn = lds + (tn & 3) * G::BUF;   // behind the last block: what is there, for nothing
         frag pf[NQ][2];
         float top[NQ];
+        u32x4 vf[DB][2];
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) vf[d][ks] = value_at(Vt, krow, d, ks);
         scores(Kn, krow_n, next);
         weights(now, pf);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {              // read beside the scores' products, not after them
+            if constexpr (G::WAVES == 1) asm volatile("" : "+a"(vf[d][ks]));
+            else asm volatile("" : "+v"(vf[d][ks]));
+          }
         const bool more = j + 1 < mine;
         if (more && key_n + 32 > lim_least) mask(Kn + G::TILE, krow_n, key_n, next);
-        values(Vt, krow, now, pf);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int b = 0; b < NQ; ++b) o[b][d] = N::mfma(__builtin_bit_cast(frag, vf[d][ks]), pf[b][ks], o[b][d]);
         maxima(next, top);
         if (more) rescale(top);
       };
