@@ -193,19 +193,45 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave % WQ, wk = wave / WQ;
 
-  // block -> (pair of sequence and key head, tile of rows, part of the keys).  Blocks go to the 8 XCDs in turn; each XCD
-  // gets a contiguous eighth of the pairs (pairs are taken `replicas` times to make their number divisible by 8), so the
-  // blocks that share K and V share an L2; `together` pairs take turns, tile by tile.
+  // block -> (pair of sequence and key head, tile of rows, part of the keys).  Blocks go to the 8 XCDs in turn; every eighth
+  // pair belongs to an XCD (pairs are taken `replicas` times to make their number divisible by 8), so that the blocks which share
+  // K and V share an L2 and each XCD has its share of every sequence; `together` pairs take turns, tile by tile.  Their order
+  // turns by one from tile to tile: an XCD deals its blocks to four shader engines in turn, and a fixed order of pairs of
+  // different lengths would give the long ones to the same engine every time.
   const unsigned per_xcd = (unsigned)(a.pairs * a.replicas) / 8, units = (unsigned)(a.tiles * a.splits);
   const unsigned id = blockIdx.x / 8, first = id / (a.together * units) * a.together;
   const unsigned width = min((unsigned)a.together, per_xcd - first), in_group = id - first * units;
-  const unsigned vp = (blockIdx.x % 8) * per_xcd + first + in_group % width;
   const int unit = (int)(in_group / width);
+  const unsigned vp = (first + (in_group + unit) % width) * 8 + blockIdx.x % 8;
   const int split = unit % a.splits;
   const int pair = (int)(vp / (unsigned)a.replicas), replica = (int)(vp % (unsigned)a.replicas);
-  const int seq = pair % a.sequences, kvh = pair / a.sequences;
-  const int q0 = min(max(a.starts_q[seq], 0), a.tokens_q), q1 = min(max(a.starts_q[seq + 1], q0), a.tokens_q);
-  const int k0 = min(max(a.starts_k[seq], 0), a.tokens_k), k1 = min(max(a.starts_k[seq + 1], k0), a.tokens_k);
+  const int kvh = pair % a.kv_heads;
+  int seq = pair / a.kv_heads, q0, q1, k0, k1;
+  if (a.sequences > 1 && a.sequences <= 64) {
+    // the sequence with the seq-th most keys: long ones first, so that the last blocks to run are the short ones
+    const int s = min(lane, a.sequences - 1);
+    const int qf = a.starts_q[s], qt = a.starts_q[s + 1], kf = a.starts_k[s], kt = a.starts_k[s + 1];
+    const int vq0 = min(max(qf, 0), a.tokens_q), vq1 = min(max(qt, vq0), a.tokens_q);
+    const int vk0 = min(max(kf, 0), a.tokens_k), vk1 = min(max(kt, vk0), a.tokens_k);
+    const int keys = vk1 - vk0, all = __builtin_amdgcn_readfirstlane(keys);
+    if (__builtin_amdgcn_ballot_w64(keys != all)) {
+      int place = 0;
+      for (int i = 0; i < a.sequences; ++i) {
+        const int other = __builtin_amdgcn_readlane(keys, i);
+        place += other > keys || (other == keys && i < lane);
+      }
+      seq = __builtin_ctzll(__builtin_amdgcn_ballot_w64(place == seq && lane < a.sequences));
+    }
+    q0 = __builtin_amdgcn_readlane(vq0, seq);
+    q1 = __builtin_amdgcn_readlane(vq1, seq);
+    k0 = __builtin_amdgcn_readlane(vk0, seq);
+    k1 = __builtin_amdgcn_readlane(vk1, seq);
+  } else {
+    q0 = min(max(a.starts_q[seq], 0), a.tokens_q);
+    q1 = min(max(a.starts_q[seq + 1], q0), a.tokens_q);
+    k0 = min(max(a.starts_k[seq], 0), a.tokens_k);
+    k1 = min(max(a.starts_k[seq + 1], k0), a.tokens_k);
+  }
   const int nq = q1 - q0, nk = k1 - k0, rows = nq * a.group;
   if (a.clear && unit == 0 && replica == 0) {                              // what lies before the first and behind the last sequence
     const int width = a.group * a.dim;
@@ -635,7 +661,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttArgs a) {
 }
 
 // ---- the launch plan: what ac_attention_packed and its workspace size agree on
-struct Plan { int kind, rows, tiles, splits, chunk, keys; };   // kind 0: 256 rows, 1: 128 rows, 2: 32 rows and split keys
+struct Plan { int kind, rows, tiles, splits, chunk, keys; };   // kind 0: 256 rows, 1: 128 rows, 2: 32 rows and split keys, 3: 128 rows on two waves
 
 template <class T> int plan_steps(int dim) {                    // NS of the instance that holds `dim`
   const int per = 32 / (int)sizeof(T), need = (dim + per - 1) / per;
@@ -653,7 +679,11 @@ Plan make_plan(const ac_attention_args* p) {
   const int bytes = p->dim * (wide ? 4 : 2);
   Plan r;
   r.kind = rows <= 32 ? 2 : (wide || bytes > 256 || pairs * ((rows + 255) / 256) < 2 * ac_device_cus()) ? 1 : 0;
-  r.rows = r.kind == 2 ? 32 : r.kind == 1 ? 128 : 256;
+  // Heads of more than 128 bytes have one wave on a SIMD: blocks of two waves halve what is left over at the end of sequences and
+  // of the launch, for twice the transfers.  8 prompts of 1 .. 4096, 32 / 8 heads of 128 (1700 blocks of 256 rows): 457 -> 431 us;
+  // 8 prompts of 4096 (4096 blocks): 1196 -> 1222 us.
+  if (r.kind == 0 && bytes > 128 && p->tokens_q * (int64_t)p->heads / 256 < 8 * ac_device_cus()) r.kind = 3;
+  r.rows = r.kind == 2 ? 32 : r.kind != 0 ? 128 : 256;
   r.keys = r.kind == 2 ? (bytes > 512 ? 64 : 128) : 64;
   r.tiles = (int)((rows + r.rows - 1) / r.rows);
   // the key axis is split where the rows alone would leave CUs idle, into parts of 512 keys or more
@@ -681,6 +711,7 @@ int launch_kind(const AttArgs& a, int kind, hipStream_t stream) {
   constexpr bool big = NS * 32 > 256;                            // rows of more than 256 bytes: smaller tiles
   if constexpr (!Num<T>::wide && !big) {
     if (kind == 0) return launch<T, NS, 2, 4, 1, 2>(a, stream);
+    if (kind == 3) return launch<T, NS, 2, 2, 1, 1>(a, stream);
   }
   if (kind == 2) {
     if constexpr (NS * 32 > 512) return launch<T, NS, 1, 1, 1, 1>(a, stream);

@@ -8,6 +8,7 @@ return code raises.
 import ctypes
 import math
 import os
+import struct
 import threading
 
 import torch
@@ -103,12 +104,12 @@ SIGNATURES = {
     "ac_pdist": (_i, [_vp, _i64, _i, _vp, _vp]),
     "ac_ward_workspace_bytes": (_sz, [_i64]),
     "ac_ward_linkage": (_i, [_vp, _i64, _vp, _vp, _vp, _sz, _vp]),
-    "ac_rotary": (_i, [_c.POINTER(RotaryArgs), _vp]),
-    "ac_attention_packed_workspace_bytes": (_sz, [_c.POINTER(AttentionArgs)]),
-    "ac_attention_packed": (_i, [_c.POINTER(AttentionArgs), _vp, _sz, _vp]),
-    "ac_layer_norm": (_i, [_c.POINTER(NormArgs), _vp]),
-    "ac_layer_norm_backward_workspace_bytes": (_sz, [_c.POINTER(NormArgs)]),
-    "ac_layer_norm_backward": (_i, [_c.POINTER(NormArgs), _vp, _sz, _vp]),
+    "ac_rotary": (_i, [_vp, _vp]),
+    "ac_attention_packed_workspace_bytes": (_sz, [_vp]),
+    "ac_attention_packed": (_i, [_vp, _vp, _sz, _vp]),
+    "ac_layer_norm": (_i, [_vp, _vp]),
+    "ac_layer_norm_backward_workspace_bytes": (_sz, [_vp]),
+    "ac_layer_norm_backward": (_i, [_vp, _vp, _sz, _vp]),
     "ac_cluster_scores": (_i, [_vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp]),
 }
 
@@ -854,36 +855,77 @@ def cluster_scores(labels_true, labels_pred, k_true, k_pred):
 
 
 # ---------------------------------------------------------- packed sequences
+# A call of these operators on a handful of tokens takes the GPU a few microseconds, so the wrappers are written for their own
+# time too: each attribute of a tensor is fetched once, the arguments are packed in one go (struct, the layout of the C
+# structures above), and the device is switched only where it is another than the current one.
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 _LAYOUTS = {"half": ROTARY_HALF, "interleaved": ROTARY_INTERLEAVED}
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_CODES = {_vp: "P", _i64: "q", _i: "i", _f: "f"}
+
+
+def _packer(structure):
+    """struct.Struct.pack with the layout of a ctypes structure (checked against it)."""
+    flat = []
+    for _, kind in structure._fields_:
+        flat += [kind._type_] * kind._length_ if hasattr(kind, "_length_") else [kind]
+    packed = struct.Struct("@" + "".join(_CODES[k] for k in flat) + "0P")
+    assert packed.size == _c.sizeof(structure)
+    return packed.pack
+
+
+_pack_rotary, _pack_attention, _pack_norm = _packer(RotaryArgs), _packer(AttentionArgs), _packer(NormArgs)
+
+
+def _launch(device, fn, *args):
+    """An entry point on a tensor's device and that device's current stream."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        rc = fn(*args, _raw_stream(index))
+    if rc:
+        _check(rc)
+
+
+try:
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+def _no_cpu(t, name):
+    raise RuntimeError("%s must be a tensor on the HIP device (got %s); the MI355X path has no CPU fallback" % (name, getattr(t, "device", type(t))))
 
 
 def _heads(t, name, like=None):
-    """A [tokens, heads, dim] device tensor with neighbouring entries, of `like`'s type, device and dim."""
+    """Checks a [tokens, heads, dim] device tensor with neighbouring entries, of `like`'s (dtype, device, dim); -> shape, strides."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise RuntimeError("%s must be a tensor on the HIP device (got %s); the MI355X path has no CPU fallback"
-                           % (name, getattr(t, "device", type(t))))
-    if t.dim() != 3:
-        raise ValueError("%s must be [tokens, heads, dim], got %s" % (name, tuple(t.shape)))
-    if t.dtype not in _TYPES:
-        raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
-    if t.shape[2] > 1 and t.stride(2) != 1:
-        raise ValueError("%s: the entries of a head must be neighbours (stride 1), got stride %d" % (name, t.stride(2)))
-    if torch.is_grad_enabled() and t.requires_grad:
+        _no_cpu(t, name)
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3:
+        raise ValueError("%s must be [tokens, heads, dim], got %s" % (name, tuple(shape)))
+    if strides[2] != 1 and shape[2] > 1:
+        raise ValueError("%s: the entries of a head must be neighbours (stride 1), got stride %d" % (name, strides[2]))
+    if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("%s requires a gradient: this operator has no backward pass (use torch.no_grad() or detach())" % name)
-    if like is not None:
-        if t.dtype != like.dtype:
-            raise TypeError("%s is %s, but q is %s" % (name, t.dtype, like.dtype))
-        if t.device != like.device:
-            raise ValueError("%s is on %s, but q is on %s" % (name, t.device, like.device))
-        if t.shape[2] != like.shape[2]:
-            raise ValueError("%s has heads of %d, but q of %d" % (name, t.shape[2], like.shape[2]))
-    return t
+    if like is None:
+        if t.dtype not in _TYPES:
+            raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    else:
+        if t.dtype != like[0]:
+            raise TypeError("%s is %s, but q is %s" % (name, t.dtype, like[0]))
+        if t.device != like[1]:
+            raise ValueError("%s is on %s, but q is on %s" % (name, t.device, like[1]))
+        if shape[2] != like[2]:
+            raise ValueError("%s has heads of %d, but q of %d" % (name, shape[2], like[2]))
+    return shape, strides
 
 
 def _whole(t, dtypes, name, device):
-    """A contiguous device tensor of one of `dtypes` on `device`."""
+    """Checks a contiguous device tensor of one of `dtypes` on `device`."""
     if not isinstance(t, torch.Tensor) or t.device != device:
         raise RuntimeError("%s must be a tensor on %s (got %s)" % (name, device, getattr(t, "device", type(t))))
     if t.dtype not in dtypes:
@@ -903,31 +945,30 @@ def _same_view(a, b):
     return a.data_ptr() == b.data_ptr() and a.shape == b.shape and all(n <= 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
 
 
+def _disjoint(a, b):
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a1 <= b0 or b1 <= a0
+
+
 def _apart(a, b):
     """No entry of `a` is one of `b`: their spans do not meet, or both are head ranges of the same rows (slices of one buffer)."""
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    if a1 <= b0 or b1 <= a0:
+    if _disjoint(a, b):
         return True
     if a.stride(0) != b.stride(0) or a.element_size() != b.element_size():
         return False
     pitch = a.stride(0) * a.element_size()
     rows = [(lambda s: s[1] - s[0])(_span(t[:1])) for t in (a, b)]           # bytes of one token's entries
-    d = (b0 - a0) % pitch if pitch else 0
+    d = (_span(b)[0] - _span(a)[0]) % pitch if pitch else 0
     return pitch > 0 and d >= rows[0] and d + rows[1] <= pitch
 
 
 def _writable(t, name):
-    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) or not _rows_apart(t):
-        raise ValueError("%s: its entries overlap each other (strides %s)" % (name, tuple(t.stride())))
-
-
-def _rows_apart(t):
+    """Refuses a tensor whose entries share memory."""
     reach = 1
-    for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda x: x[1]):
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
         if s < reach:
-            return False
-        reach = s * (n - 1) + reach
-    return True
+            raise ValueError("%s: its entries overlap each other (strides %s)" % (name, tuple(t.stride())))
+        reach += s * (n - 1)
 
 
 def sequence_starts(lengths, device):
@@ -970,52 +1011,63 @@ def rotary(q, k, positions, frequencies, layout="half", offset=0, amplitude=1.0,
     positions: int32 / int64 [tokens] or [axes, tokens]; frequencies: fp64 [axes, part / 2 / axes] (or [part / 2]) on the
     device (rotary_frequencies).  inverse=True turns back by the same angles (the transpose of the map: its gradient).
     out_q / out_k: where to write; q / k themselves turn in place.  Returns out_q, or (out_q, out_k) with k."""
-    _heads(q, "q")
+    shape, qs = _heads(q, "q")
+    tokens, heads, dim = shape
+    dtype, device = q.dtype, q.device
+    like = (dtype, device, dim)
     if layout not in _LAYOUTS:
         raise ValueError("layout must be 'half' or 'interleaved', got %r" % (layout,))
-    tokens, heads, dim = q.shape
+    kv_heads, ks, kp = 0, (0, 0), 0
     if k is not None:
-        _heads(k, "k", q)
-        if k.shape[0] != tokens:
-            raise ValueError("k has %d tokens, but q has %d" % (k.shape[0], tokens))
+        kshape, ks = _heads(k, "k", like)
+        if kshape[0] != tokens:
+            raise ValueError("k has %d tokens, but q has %d" % (kshape[0], tokens))
+        kv_heads, kp = kshape[1], k.data_ptr()
+        if kv_heads == 0:
+            raise ValueError("q and k need a head each")
     elif out_k is not None:
         raise ValueError("out_k without k")
-    _whole(frequencies, (torch.float64,), "frequencies", q.device)
-    if frequencies.dim() not in (1, 2):
-        raise ValueError("frequencies must be [axes, pairs] or [pairs], got %s" % (tuple(frequencies.shape),))
-    axes = frequencies.shape[0] if frequencies.dim() == 2 else 1
-    _whole(positions, (torch.int32, torch.int64), "positions", q.device)
-    if tuple(positions.shape) not in ((axes, tokens),) + (((tokens,),) if axes == 1 else ()):
-        raise ValueError("positions must be [%d, %d]%s, got %s" % (axes, tokens, " or [%d]" % tokens if axes == 1 else "", tuple(positions.shape)))
-    a = RotaryArgs()
-    outs = []
-    for i, (x, out, name) in enumerate(((q, out_q, "out_q"), (k, out_k, "out_k"))):
-        if x is None:
-            continue
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        else:
-            _heads(out, name, q)
-            if out.shape != x.shape:
-                raise ValueError("%s must be %s, got %s" % (name, tuple(x.shape), tuple(out.shape)))
-            _writable(out, name)
-            for other, other_name in ((q, "q"), (k, "k")):
-                if other is not None and not _apart(out, other) and not (other is x and _same_view(out, x)):
-                    raise ValueError("%s overlaps %s" % (name, other_name))
-            if outs and not _apart(out, outs[0]):
-                raise ValueError("out_k overlaps out_q")
-        outs.append(out)
-        a.src[i], a.dst[i], a.heads[i] = x.data_ptr(), out.data_ptr(), x.shape[1]
-        a.src_token[i], a.src_head[i], a.dst_token[i], a.dst_head[i] = x.stride(0), x.stride(1), out.stride(0), out.stride(1)
-    a.positions, a.position_axis, a.positions64 = positions.data_ptr(), tokens, int(positions.dtype == torch.int64)
-    a.frequencies = frequencies.data_ptr()
-    a.tokens, a.type, a.layout, a.dim, a.part = tokens, _TYPES[q.dtype], _LAYOUTS[layout], dim, 2 * frequencies.numel()
-    a.offset, a.axes, a.inverse, a.amplitude = int(offset), axes, int(bool(inverse)), float(amplitude)
-    if heads == 0 or (k is not None and k.shape[1] == 0):
+    if heads == 0:
         raise ValueError("q and k need a head each")
-    with torch.cuda.device(q.device):
-        _check(lib().ac_rotary(_c.byref(a), _stream()))
-    return outs[0] if k is None else (outs[0], outs[1])
+    _whole(frequencies, (torch.float64,), "frequencies", device)
+    _whole(positions, (torch.int32, torch.int64), "positions", device)
+    fshape, pshape = frequencies.shape, positions.shape
+    if len(fshape) not in (1, 2):
+        raise ValueError("frequencies must be [axes, pairs] or [pairs], got %s" % (tuple(fshape),))
+    axes = fshape[0] if len(fshape) == 2 else 1
+    if pshape != (axes, tokens) and not (axes == 1 and pshape == (tokens,)):
+        raise ValueError("positions must be [%d, %d]%s, got %s" % (axes, tokens, " or [%d]" % tokens if axes == 1 else "", tuple(pshape)))
+    if out_q is None:
+        out_q = q.new_empty(shape)
+        os = (heads * dim, dim)
+    else:
+        os = _rotary_out(out_q, "out_q", q, like, q, k)
+    kos = (0, 0)
+    if k is not None:
+        if out_k is None:
+            out_k = k.new_empty(kshape)
+            kos = (kv_heads * dim, dim)
+        else:
+            kos = _rotary_out(out_k, "out_k", k, like, q, k)
+            if not _apart(out_k, out_q):
+                raise ValueError("out_k overlaps out_q")
+    pairs = frequencies.numel()
+    _launch(device, lib().ac_rotary, _pack_rotary(
+        q.data_ptr(), kp, out_q.data_ptr(), out_k.data_ptr() if k is not None else 0, qs[0], ks[0], qs[1], ks[1], os[0], kos[0], os[1], kos[1],
+        heads, kv_heads, positions.data_ptr(), tokens, positions.dtype == torch.int64, frequencies.data_ptr(), tokens, _TYPES[dtype],
+        _LAYOUTS[layout], dim, 2 * pairs, offset, axes, bool(inverse), amplitude))
+    return out_q if k is None else (out_q, out_k)
+
+
+def _rotary_out(out, name, x, like, q, k):
+    shape, strides = _heads(out, name, like)
+    if shape != x.shape:
+        raise ValueError("%s must be %s, got %s" % (name, tuple(x.shape), tuple(shape)))
+    _writable(out, name)
+    for other, other_name in ((q, "q"), (k, "k")):
+        if other is not None and not _apart(out, other) and not (other is x and _same_view(out, x)):
+            raise ValueError("%s overlaps %s" % (name, other_name))
+    return strides
 
 
 def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, causal=False, scale=None, out=None, want_sums=False):
@@ -1029,97 +1081,109 @@ def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, c
     were in `out` (without `out`: zero).  scale: 1 / sqrt(dim) unless given.  want_sums: also the fp32 [tokens, heads] logarithm of
     each row's sum of exponentials (-inf for a row that sees no key, and outside every sequence).
     Tensors whose heads do not start at multiples of 16 bytes are copied first."""
-    _heads(q, "q")
-    _heads(k, "k", q)
-    _heads(v, "v", q)
-    tokens, heads, dim = q.shape
-    if k.shape != v.shape:
-        raise ValueError("k is %s, but v is %s" % (tuple(k.shape), tuple(v.shape)))
+    shape, qs = _heads(q, "q")
+    tokens, heads, dim = shape
+    dtype, device = q.dtype, q.device
+    like = (dtype, device, dim)
+    kshape, ks = _heads(k, "k", like)
+    vshape, vs = _heads(v, "v", like)
+    if kshape != vshape:
+        raise ValueError("k is %s, but v is %s" % (tuple(kshape), tuple(vshape)))
+    keys, kv_heads, _ = kshape
+    _whole(starts_q, (torch.int32,), "starts_q", device)
     if starts_k is None:
         starts_k = starts_q
-        if k.shape[0] != tokens:
-            raise ValueError("k has %d tokens and q %d: starts_k is needed" % (k.shape[0], tokens))
-    for t, name in ((starts_q, "starts_q"), (starts_k, "starts_k")):
-        _whole(t, (torch.int32,), name, q.device)
-        if t.dim() != 1 or t.shape[0] < 1:
-            raise ValueError("%s must be [sequences + 1], got %s" % (name, tuple(t.shape)))
-    if starts_q.shape != starts_k.shape:
-        raise ValueError("starts_q speaks of %d sequences, starts_k of %d" % (starts_q.shape[0] - 1, starts_k.shape[0] - 1))
+        if keys != tokens:
+            raise ValueError("k has %d tokens and q %d: starts_k is needed" % (keys, tokens))
+    else:
+        _whole(starts_k, (torch.int32,), "starts_k", device)
+    count = starts_q.shape
+    if len(count) != 1 or count[0] < 1:
+        raise ValueError("starts_q must be [sequences + 1], got %s" % (tuple(count),))
+    if starts_k.shape != count:
+        raise ValueError("starts_q is %s, but starts_k is %s" % (tuple(count), tuple(starts_k.shape)))
+    sequences = count[0] - 1
     clear = out is None
     if clear:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
+        os = (heads * dim, dim)
     else:
-        _heads(out, "out", q)
-        if out.shape != q.shape:
-            raise ValueError("out must be %s, got %s" % (tuple(q.shape), tuple(out.shape)))
+        _, os = _heads(out, "out", like)
+        if out.shape != shape:
+            raise ValueError("out must be %s, got %s" % (tuple(shape), tuple(out.shape)))
         _writable(out, "out")
         for t, name in ((q, "q"), (k, "k"), (v, "v")):
             if not _apart(out, t):
                 raise ValueError("out overlaps %s" % name)
         if not _aligned(out):
             raise ValueError("out: every head must start at a multiple of 16 bytes")
-    q, k, v = (t if _aligned(t) else t.contiguous() if _aligned(t.contiguous()) else t.clone() for t in (q, k, v))
-    sums = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if want_sums else None
-    if starts_q.shape[0] == 1:                             # no sequence at all
+    sums = q.new_empty((tokens, heads), dtype=torch.float32) if want_sums else None
+    if sequences == 0:
         if clear:
             out.zero_()
         if want_sums:
             sums.fill_(-math.inf)
         return (out, sums) if want_sums else out
-    a = AttentionArgs()
-    a.q, a.k, a.v, a.out, a.sums = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), sums.data_ptr() if want_sums else None
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
-        for i, what in enumerate(("token", "head")):        # the stride of an axis of one says nothing
-            setattr(a, "%s_%s" % (name, what), t.stride(i) if t.shape[i] > 1 else 0)
-    a.starts_q, a.starts_k, a.sequences = starts_q.data_ptr(), starts_k.data_ptr(), starts_q.shape[0] - 1
-    a.tokens_q, a.tokens_k, a.heads, a.kv_heads, a.dim = tokens, k.shape[0], heads, k.shape[1], dim
-    a.max_q, a.max_k = tokens if max_q is None else int(max_q), k.shape[0] if max_k is None else int(max_k)
-    a.causal, a.clear, a.type, a.scale = int(bool(causal)), int(clear) | 2 * int(want_sums), _TYPES[q.dtype], float(dim ** -0.5 if scale is None else scale)
-    with torch.cuda.device(q.device):
-        n = lib().ac_attention_packed_workspace_bytes(_c.byref(a))
-        # of its own for every call: two graphs captured on one stream must not share the parts of a split key axis
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        _check(lib().ac_attention_packed(_c.byref(a), ws.data_ptr() if n else None, n, _stream()))
+    size = 4 if dtype == torch.float32 else 2
+    qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (qp | kp | vp | (qs[0] | qs[1] | ks[0] | ks[1] | vs[0] | vs[1]) * size) & 15:
+        q, k, v = (t if _aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+        qp, kp, vp, qs, ks, vs = q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q), _strides(k), _strides(v)
+        os = _strides(out)
+    if keys == 1:
+        ks, vs = (0, ks[1]), (0, vs[1])
+    args = _pack_attention(qp, kp, vp, out.data_ptr(), sums.data_ptr() if want_sums else 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
+                           starts_q.data_ptr(), starts_k.data_ptr(), tokens, keys, sequences, heads, kv_heads, dim,
+                           tokens if max_q is None else max_q, keys if max_k is None else max_k, bool(causal), clear + 2 * want_sums,
+                           _TYPES[dtype], dim ** -0.5 if scale is None else scale)
+    handle = lib()
+    n = handle.ac_attention_packed_workspace_bytes(args)
+    # of its own for every call: two graphs captured on one stream must not share the parts of a split key axis
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
+    _launch(device, handle.ac_attention_packed, args, ws.data_ptr() if n else None, n)
     return (out, sums) if want_sums else out
+
+
+def _strides(t):
+    """Strides of the tokens and heads; that of an axis of one says nothing and counts as 0."""
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape[:2], t.stride()[:2]))
 
 
 def _aligned(t):
     """Every head starts at a multiple of 16 bytes, as the kernels load them."""
     size = t.element_size()
-    return t.data_ptr() % 16 == 0 and all(n <= 1 or s * size % 16 == 0 for n, s in zip(t.shape[:2], t.stride()[:2]))
+    return t.data_ptr() % 16 == 0 and all(s * size % 16 == 0 for s in _strides(t))
 
 
 def _rows(t, name, like=None):
     """`t` [..., width] as [rows, width] with neighbouring entries (a copy only where its axes do not fold into one stride)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise RuntimeError("%s must be a tensor on the HIP device (got %s); the MI355X path has no CPU fallback"
-                           % (name, getattr(t, "device", type(t))))
-    if t.dim() < 1 or t.shape[-1] < 1:
-        raise ValueError("%s must be [..., width], got %s" % (name, tuple(t.shape)))
-    if t.dtype not in _TYPES:
-        raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
-    if torch.is_grad_enabled() and t.requires_grad:
+        _no_cpu(t, name)
+    shape = t.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError("%s must be [..., width], got %s" % (name, tuple(shape)))
+    if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("%s requires a gradient: this operator records no graph (layer_norm_backward has the gradients)" % name)
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError("%s is %s %s on %s, but x is %s %s on %s" % (name, t.dtype, tuple(t.shape), t.device, like.dtype, tuple(like.shape), like.device))
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
+    if like is None:
+        if t.dtype not in _TYPES:
+            raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    elif shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError("%s is %s %s on %s, but x is %s %s on %s" % (name, t.dtype, tuple(shape), t.device, like.dtype, tuple(like.shape), like.device))
+    if len(shape) != 2:
+        t = t.reshape(-1, shape[-1])
+    return t if t.stride(1) == 1 or shape[-1] == 1 else t.contiguous()
 
 
-def _norm_vector(t, name, x):
-    if not isinstance(t, torch.Tensor) or t.device != x.device:
-        raise RuntimeError("%s must be a tensor on %s (got %s)" % (name, x.device, getattr(t, "device", type(t))))
-    if tuple(t.shape) != (x.shape[-1],):
-        raise ValueError("%s must be [%d], got %s" % (name, x.shape[-1], tuple(t.shape)))
-    if t.dtype not in (x.dtype, torch.float32):
-        raise TypeError("%s must be %s or float32, got %s" % (name, x.dtype, t.dtype))
-    if torch.is_grad_enabled() and t.requires_grad:
+def _norm_vector(t, name, x, dtype, device, width):
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise RuntimeError("%s must be a tensor on %s (got %s)" % (name, device, getattr(t, "device", type(t))))
+    if t.shape != (width,):
+        raise ValueError("%s must be [%d], got %s" % (name, width, tuple(t.shape)))
+    if t.dtype != dtype and t.dtype != torch.float32:
+        raise TypeError("%s must be %s or float32, got %s" % (name, dtype, t.dtype))
+    if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("%s requires a gradient: this operator records no graph (layer_norm_backward has the gradients)" % name)
-    return t.contiguous()
-
-
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return t if t.stride(0) == 1 or width == 1 else t.contiguous()
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, want_stats=False):
@@ -1127,30 +1191,36 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, want_stats=False):
     weight and bias [width] in x's type or float32 (both the same), or None.  out: where to write (x itself is allowed).
     want_stats: also the fp32 mean and 1 / standard deviation of each row, which layer_norm_backward takes."""
     rows = _rows(x, "x")
-    weight = None if weight is None else _norm_vector(weight, "weight", x)
-    bias = None if bias is None else _norm_vector(bias, "bias", x)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError("weight is %s, but bias is %s" % (weight.dtype, bias.dtype))
+    dtype, device = x.dtype, x.device
+    count, width = rows.shape
+    kind = torch.float32
+    if bias is not None:
+        bias = _norm_vector(bias, "bias", x, dtype, device, width)
+        kind = bias.dtype
+    if weight is not None:
+        weight = _norm_vector(weight, "weight", x, dtype, device, width)
+        kind = weight.dtype
+        if bias is not None and bias.dtype != kind:
+            raise TypeError("weight is %s, but bias is %s" % (kind, bias.dtype))
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    to = _rows(out, "out", x)
-    if to.data_ptr() != out.data_ptr():
-        raise ValueError("out: its axes must fold into rows of one stride, entries neighbours (strides %s)" % (tuple(out.stride()),))
-    _writable(out, "out")
-    for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
-        if t is not None and not _disjoint(out, t) and not (t is x and _same_view(out, x)):
-            raise ValueError("out overlaps %s" % name)
-    a = NormArgs()
-    a.x, a.y, a.x_row, a.y_row = rows.data_ptr(), to.data_ptr(), _row_stride(rows), _row_stride(to)
-    a.weight, a.bias = None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr()
-    a.rows, a.width, a.type, a.eps = rows.shape[0], rows.shape[1], _TYPES[x.dtype], float(eps)
-    a.weight_type = _TYPES[next((t.dtype for t in (weight, bias) if t is not None), torch.float32)]
+        out = x.new_empty(x.shape)
+        out_row, to = width, out
+    else:
+        to = _rows(out, "out", x)
+        if to.data_ptr() != out.data_ptr():
+            raise ValueError("out: its axes must fold into rows of one stride, entries neighbours (strides %s)" % (tuple(out.stride()),))
+        _writable(out, "out")
+        for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
+            if t is not None and not _disjoint(out, t) and not (t is x and _same_view(out, x)):
+                raise ValueError("out overlaps %s" % name)
+        out_row = to.stride(0)
     mean = rstd = None
     if want_stats:
-        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
-        a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
-    with torch.cuda.device(x.device):
-        _check(lib().ac_layer_norm(_c.byref(a), _stream()))
+        mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _launch(device, lib().ac_layer_norm, _pack_norm(
+        rows.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(), to.data_ptr(), 0, 0, 0, 0,
+        mean.data_ptr() if want_stats else 0, rstd.data_ptr() if want_stats else 0, rows.stride(0) if count > 1 else width,
+        out_row if count > 1 else width, 0, 0, count, width, _TYPES[dtype], _TYPES[kind], eps))
     return (out, mean, rstd) if want_stats else out
 
 
@@ -1158,27 +1228,24 @@ def layer_norm_backward(dy, x, weight, mean, rstd, want=(True, True, True)):
     """Gradients of layer_norm at x: (dx, dweight, dbias), in x's and the weight's type (float32 without a weight); mean and rstd as
     layer_norm(want_stats=True) returned them.  want: which of the three to compute (None in place of the others)."""
     rows, grads = _rows(x, "x"), _rows(dy, "dy", x)
-    weight = None if weight is None else _norm_vector(weight, "weight", x)
+    dtype, device = x.dtype, x.device
+    count, width = rows.shape
+    kind = torch.float32
+    if weight is not None:
+        weight = _norm_vector(weight, "weight", x, dtype, device, width)
+        kind = weight.dtype
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        _whole(t, (torch.float32,), name, x.device)
+        _whole(t, (torch.float32,), name, device)
         if t.shape != x.shape[:-1]:
             raise ValueError("%s must be %s, got %s" % (name, tuple(x.shape[:-1]), tuple(t.shape)))
-    kind = torch.float32 if weight is None else weight.dtype
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want[0] else None
-    dw, db = (torch.empty(rows.shape[1], dtype=kind, device=x.device) if w else None for w in want[1:])
-    a = NormArgs()
-    a.x, a.dy, a.x_row, a.dy_row, a.dx_row = rows.data_ptr(), grads.data_ptr(), _row_stride(rows), _row_stride(grads), rows.shape[1]
-    a.weight, a.mean, a.rstd = None if weight is None else weight.data_ptr(), mean.data_ptr(), rstd.data_ptr()
-    for name, t in (("dx", dx), ("dweight", dw), ("dbias", db)):
-        setattr(a, name, None if t is None else t.data_ptr())
-    a.rows, a.width, a.type, a.weight_type = rows.shape[0], rows.shape[1], _TYPES[x.dtype], _TYPES[kind]
-    with torch.cuda.device(x.device):
-        n = lib().ac_layer_norm_backward_workspace_bytes(_c.byref(a))
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None       # of this call alone, as in attention_packed
-        _check(lib().ac_layer_norm_backward(_c.byref(a), ws.data_ptr() if n else None, n, _stream()))
+    dx = x.new_empty(x.shape) if want[0] else None
+    dw = x.new_empty(width, dtype=kind) if want[1] else None
+    db = x.new_empty(width, dtype=kind) if want[2] else None
+    args = _pack_norm(rows.data_ptr(), 0 if weight is None else weight.data_ptr(), 0, 0, grads.data_ptr(), 0 if dx is None else dx.data_ptr(),
+                      0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                      rows.stride(0) if count > 1 else width, 0, grads.stride(0) if count > 1 else width, width, count, width, _TYPES[dtype], _TYPES[kind], 0.0)
+    handle = lib()
+    n = handle.ac_layer_norm_backward_workspace_bytes(args)
+    ws = x.new_empty(n, dtype=torch.uint8) if n else None       # of this call alone, as in attention_packed
+    _launch(device, handle.ac_layer_norm_backward, args, ws.data_ptr() if n else None, n)
     return dx, dw, db
-
-
-def _disjoint(a, b):
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a1 <= b0 or b1 <= a0
