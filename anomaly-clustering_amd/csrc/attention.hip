@@ -617,15 +617,16 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
   }
 }
 
-// Joins the parts of a split key axis: one wave per row, lane -> entries.
+// Joins the parts of a split key axis: a block per row; eight groups of 32 lanes take every eighth part, lane -> four entries (and four
+// more, up to 256).  The parts' maxima and sums: lane -> part.
 template <class T>
 __global__ __launch_bounds__(256) void join_kernel(const AttArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.tokens_q * a.heads) return;
+  __shared__ float weight[64], all[8][260];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t row = blockIdx.x;
   const int token = (int)(row / a.heads), hh = (int)(row - (int64_t)token * a.heads);
   // the sequence that holds the token: the first whose (clamped, as above) range does
-  int seq = -1, nk = 0;
+  int seq = -1;
   for (int s0 = 0; s0 < a.sequences && seq < 0; s0 += 64) {
     const int s = s0 + lane;
     bool here = false;
@@ -636,28 +637,45 @@ __global__ __launch_bounds__(256) void join_kernel(const AttArgs a) {
     const unsigned long long m = __builtin_amdgcn_ballot_w64(here);
     if (m) seq = s0 + __builtin_ctzll(m);
   }
-  if (seq < 0) return;                                           // behind the last sequence: left as it is
-  const int k0 = min(max(a.starts_k[seq], 0), a.tokens_k);
-  nk = min(max(a.starts_k[seq + 1], k0), a.tokens_k) - k0;
-  const int parts = max(1, min(a.splits, (nk + a.chunk - 1) / a.chunk));
+  if (seq < 0) return;                                           // outside every sequence: left as it is (the whole block)
+  const int k0 = min(max(a.starts_k[seq], 0), a.tokens_k), nk = min(max(a.starts_k[seq + 1], k0), a.tokens_k) - k0;
+  const int parts = max(1, min(a.splits, (nk + a.chunk - 1) / a.chunk));            // at most 64
   const size_t step = (size_t)a.tokens_q * a.heads;
-  float m = NO_MAX;
-  for (int s = 0; s < parts; ++s) m = fmaxf(m, a.part_ml[2 * (s * step + row)]);
-  float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < parts; ++s) {
-    const size_t at = s * step + row;
-    const float c = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - m);
-    l += a.part_ml[2 * at + 1] * c;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (lane + 64 * j < a.dim) x[j] += a.part_o[at * a.dim + lane + 64 * j] * c;
+  float m = NO_MAX, l = 0.f;
+  if (lane < parts) {
+    const float* ml = a.part_ml + 2 * (lane * step + row);
+    m = ml[0];
+    l = ml[1];
   }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  T* dst = static_cast<T*>(a.out) + (int64_t)token * a.o_tok + (int64_t)hh * a.o_head;
+  const float top = wave_max(m), w = lane < parts ? __builtin_amdgcn_exp2f(m - top) : 0.f;
+  l = wave_sum(l * w);
+  if (tid < 64) weight[tid] = w;
+  __syncthreads();
+  const int grp = tid >> 5, e = (tid & 31) * 4;
+  f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
+  for (int s = grp; s < parts; s += 8) {
+    const float* p = a.part_o + (s * step + row) * a.dim;
+    const float ws = weight[s];
+    f32x4 y0 = x0, y1 = x0;
+    if (e < a.dim) y0 = *reinterpret_cast<const f32x4*>(p + e);
+    if (e + 128 < a.dim) y1 = *reinterpret_cast<const f32x4*>(p + e + 128);
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (lane + 64 * j < a.dim) dst[lane + 64 * j] = (T)(x[j] * inv);
-  if (a.sums && lane == 0) a.sums[row] = l == 0.f ? -__builtin_inff() : 0.69314718055994530942f * (m + __builtin_amdgcn_logf(l));
+    for (int j = 0; j < 4; ++j) {
+      if (e < a.dim) x0[j] += y0[j] * ws;
+      if (e + 128 < a.dim) x1[j] += y1[j] * ws;
+    }
+  }
+  *reinterpret_cast<f32x4*>(&all[grp][e]) = x0;
+  *reinterpret_cast<f32x4*>(&all[grp][e + 128]) = x1;
+  __syncthreads();
+  if (tid < a.dim) {
+    float x = 0.f;
+#pragma unroll
+    for (int g = 0; g < 8; ++g) x += all[g][tid];
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    static_cast<T*>(a.out)[(int64_t)token * a.o_tok + (int64_t)hh * a.o_head + tid] = (T)(x * inv);
+  }
+  if (a.sums && tid == 0) a.sums[row] = l == 0.f ? -__builtin_inff() : 0.69314718055994530942f * (top + __builtin_amdgcn_logf(l));
 }
 
 // ---- the launch plan: what ac_attention_packed and its workspace size agree on
@@ -684,11 +702,14 @@ Plan make_plan(const ac_attention_args* p) {
   // 8 prompts of 4096 (4096 blocks): 1196 -> 1222 us.
   if (r.kind == 0 && bytes > 128 && p->tokens_q * (int64_t)p->heads / 256 < 8 * ac_device_cus()) r.kind = 3;
   r.rows = r.kind == 2 ? 32 : r.kind != 0 ? 128 : 256;
-  r.keys = r.kind == 2 ? (bytes > 512 ? 64 : 128) : 64;
+  r.keys = r.kind == 2 && wide && bytes <= 256 ? 128 : 64;
   r.tiles = (int)((rows + r.rows - 1) / r.rows);
-  // the key axis is split where the rows alone would leave CUs idle, into parts of 512 keys or more
-  const int64_t blocks = pairs * r.tiles, want = 6LL * ac_device_cus();
-  int64_t splits = blocks >= want / 3 ? 1 : min((want + blocks - 1) / blocks, (max_k + 511) / 512);
+  // The key axis is split where the rows alone would leave CUs idle, into parts of 256 keys or more: so many that a CU gets about
+  // four (16-bit; fp32 six) blocks.  Two waves on tiles of 64 keys, 64 KB of LDS: two blocks of a CU cover each other's start and
+  // end.  16 queries on 64 .. 16000 keys, 32 / 8 heads of 128: 90 us, against 106 with four waves on 128 keys; 64 queries on 4096
+  // keys each: 183 us (5.9 TB/s) against 196.
+  const int64_t blocks = pairs * r.tiles, want = (wide ? 6LL : 4LL) * ac_device_cus();
+  int64_t splits = blocks >= want / 2 ? 1 : min((want + blocks - 1) / blocks, (max_k + 255) / 256);
   splits = max((int64_t)1, min((int64_t)64, splits));
   r.chunk = (int)(((max_k + splits - 1) / splits + r.keys - 1) / r.keys * r.keys);
   r.splits = (int)((max_k + r.chunk - 1) / r.chunk);
@@ -716,7 +737,7 @@ int launch_kind(const AttArgs& a, int kind, hipStream_t stream) {
   if (kind == 2) {
     if constexpr (NS * 32 > 512) return launch<T, NS, 1, 1, 1, 1>(a, stream);
     else if constexpr (big) return launch<T, NS, 1, 1, 2, 1>(a, stream);
-    else return launch<T, NS, 1, 1, 4, 1>(a, stream);
+    else return launch<T, NS, 1, 1, Num<T>::wide ? 4 : 2, 1>(a, stream);
   }
   if constexpr (NS * 32 > 512) return launch<T, NS, 1, 4, 1, 1>(a, stream);
   else return launch<T, NS, 1, 4, 1, big ? 1 : 2>(a, stream);
@@ -752,7 +773,7 @@ int launch_type(const AttArgs& a, int kind, hipStream_t stream) {
   if (rc != AC_OK) return rc;
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.tokens_q * a.heads;
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, stream, a);
   }
   return AC_OK;
 }

@@ -122,10 +122,14 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_forward_kernel(cons
   if (t == 0 && a.mean) { a.mean[row] = mean; a.rstd[row] = rstd; }
 }
 
+// The next row's loads are issued before this row's sums are taken, so that a block always has two rows on their way (one row at
+// a time: 133 us for 24571 x 4096 bf16, 4.5 TB/s).
 template <class T, int VEC, int N, int W>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_backward_kernel(const NormArgs a) {
   constexpr int R = W >= 4 ? 1 : 4 / W;           // rows in flight per block
+  typedef typename Pack<T, VEC>::type raw;
   __shared__ float box[W][2];
+  __shared__ float share[R > 1 ? 2 * 64 * N * VEC : 1];
   const int tid = threadIdx.x, wave = tid >> 6, t = R == 1 ? tid : tid % (64 * W), sub = R == 1 ? 0 : wave / W;
   const int chunks = a.C / VEC;
   float w[N][VEC], dw[N][VEC], db[N][VEC];
@@ -137,33 +141,45 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_backward_kernel(con
     if (a.w && c < chunks) load_w<T, VEC>(a.w, a.w32, c * VEC, w[i]);
   }
   const float inv = 1.0f / (float)a.C;
-  for (int64_t row = (int64_t)blockIdx.x * R + sub; row < a.rows; row += (int64_t)gridDim.x * R) {
+  const int64_t step = (int64_t)gridDim.x * R;
+  raw xr[N], gr[N];
+  float mean = 0.f, rstd = 0.f;
+  auto fetch = [&](int64_t row) {
     const T* x = static_cast<const T*>(a.x) + row * a.x_row;
     const T* dy = static_cast<const T*>(a.dy) + row * a.dy_row;
-    const float mean = a.mean_in[row], rstd = a.rstd_in[row];
-    float u[N][VEC], g[N][VEC], s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = t + 64 * W * i;
       if (c < chunks) {
-        load<T, VEC>(x + c * VEC, u[i]);
-        load<T, VEC>(dy + c * VEC, g[i]);
+        xr[i] = *reinterpret_cast<const raw*>(x + c * VEC);
+        gr[i] = *reinterpret_cast<const raw*>(dy + c * VEC);
       }
     }
+    mean = a.mean_in[row];
+    rstd = a.rstd_in[row];
+  };
+  int64_t row = (int64_t)blockIdx.x * R + sub;
+  if (row < a.rows) fetch(row);
+  for (; row < a.rows; row += step) {
+    float u[N][VEC], g[N][VEC], s1 = 0.f, s2 = 0.f;
+    const float r = rstd;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (t + 64 * W * i < chunks) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          u[i][j] = (u[i][j] - mean) * rstd;
-          dw[i][j] += g[i][j] * u[i][j];
-          db[i][j] += g[i][j];
-          g[i][j] *= w[i][j];
+          float xv, gv;
+          if constexpr (VEC == 1) { xv = (float)xr[i]; gv = (float)gr[i]; } else { xv = (float)xr[i][j]; gv = (float)gr[i][j]; }
+          u[i][j] = (xv - mean) * r;
+          dw[i][j] += gv * u[i][j];
+          db[i][j] += gv;
+          g[i][j] = gv * w[i][j];
           s1 += g[i][j];
           s2 += g[i][j] * u[i][j];
         }
       }
     }
+    if (row + step < a.rows) fetch(row + step);
     if (a.dx) {
       row_sum<W>(s1, s2, box, wave);
       s1 *= inv;
@@ -175,20 +191,47 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_backward_kernel(con
         if (c < chunks) {
           float o[VEC];
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) o[j] = rstd * (g[i][j] - s1 - u[i][j] * s2);
+          for (int j = 0; j < VEC; ++j) o[j] = r * (g[i][j] - s1 - u[i][j] * s2);
           store<T, VEC>(dx + c * VEC, o);
         }
       }
     }
   }
   if (!a.part) return;
-  float* p = a.part + ((size_t)blockIdx.x * R + sub) * 2 * a.C;
+  if constexpr (R > 1) {                           // the block's waves one after the other, in their order
+    for (int k = 0; k < R; ++k) {
+      if (sub == k) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const int at = (i * VEC + j) * 64 + t;
+            share[at] = k ? share[at] + dw[i][j] : dw[i][j];
+            share[64 * N * VEC + at] = k ? share[64 * N * VEC + at] + db[i][j] : db[i][j];
+          }
+      }
+      __syncthreads();
+    }
+    if (sub) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        dw[i][j] = share[(i * VEC + j) * 64 + t];
+        db[i][j] = share[64 * N * VEC + (i * VEC + j) * 64 + t];
+      }
+  }
+  float* p = a.part + (size_t)blockIdx.x * 2 * a.C;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int c = t + 64 * W * i;
     if (c < chunks) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) { p[c * VEC + j] = dw[i][j]; p[a.C + c * VEC + j] = db[i][j]; }
+      store<float, VEC < 4 ? VEC : 4>(p + c * VEC, dw[i]);
+      store<float, VEC < 4 ? VEC : 4>(p + a.C + c * VEC, db[i]);
+      if constexpr (VEC == 8) {
+        store<float, 4>(p + c * VEC + 4, dw[i] + 4);
+        store<float, 4>(p + a.C + c * VEC + 4, db[i] + 4);
+      }
     }
   }
 }
@@ -257,38 +300,47 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(const NormArgs a) {
   a.part[(size_t)blockIdx.y * 2 * a.C + a.C + c] = db;
 }
 
-// Adds the blocks' shares: 32 columns x 8 groups of blocks per block
+// Adds the blocks' shares: 32 columns x 32 groups of blocks per block, four shares in flight per thread (8 groups, one share at
+// a time: 38 us for 1024 shares of 768 columns)
 template <class T>
-__global__ __launch_bounds__(256) void norm_join_kernel(const NormArgs a) {
-  __shared__ float sums[8][33];
+__global__ __launch_bounds__(1024) void norm_join_kernel(const NormArgs a) {
+  __shared__ float sums[32][33];
   const int col = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + col;             // over 2 C: dw, then db
-  float s = 0.f;
-  if (c < 2 * a.C)
-    for (int b = grp; b < a.blocks; b += 8) s += a.part[(size_t)b * 2 * a.C + c];
-  sums[grp][col] = s;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < 2 * a.C) {
+    const float* p = a.part + c;
+    const size_t step = 2 * (size_t)a.C;
+    int b = grp;
+    for (; b + 96 < a.blocks; b += 128) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += p[(b + 32 * i) * step];
+    }
+    for (; b < a.blocks; b += 32) s[0] += p[b * step];
+  }
+  sums[grp][col] = (s[0] + s[1]) + (s[2] + s[3]);
   __syncthreads();
   if (grp || c >= 2 * a.C) return;
-  s = 0.f;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s += sums[i][col];
+  for (int i = 0; i < 32; ++i) t[i & 3] += sums[i][col];
+  const float sum = (t[0] + t[1]) + (t[2] + t[3]);
   void* out = c < a.C ? a.dw : a.db;
   const int at = c < a.C ? c : c - a.C;
   if (!out) return;
-  if (a.w32) static_cast<float*>(out)[at] = s;
-  else static_cast<T*>(out)[at] = (T)s;
+  if (a.w32) static_cast<float*>(out)[at] = sum;
+  else static_cast<T*>(out)[at] = (T)sum;
 }
 
 // ---- which instance takes a width: VEC entries per access, N accesses per thread, W waves per row; N = 0: the wide kernels
 struct Choice { int vec, n, w; };
-Choice choose(int C, int size, bool aligned) {
+Choice choose(int C, int size, bool aligned, int most) {         // most: entries of a row per thread
   Choice k;
   k.vec = aligned ? 16 / size : 1;
   const int64_t chunks = ((int64_t)C + k.vec - 1) / k.vec;
-  const int most = aligned ? 16 / k.vec : 16;       // 16 entries of a row per thread
   for (int w : {1, 4, 16}) {
     k.w = w;
-    for (int n = 1; n <= most; n *= 2) {
+    for (int n = 1; n <= most / k.vec; n *= 2) {
       k.n = n;
       if (chunks <= (int64_t)64 * w * n) return k;
     }
@@ -296,17 +348,25 @@ Choice choose(int C, int size, bool aligned) {
   k.n = 0;
   return k;
 }
-int backward_blocks(int64_t rows, int C, const Choice& k) {    // blocks of the row walk (their shares are 8 C bytes each)
-  const int per = k.n == 0 ? 1 : k.w >= 4 ? 1 : 4 / k.w;
-  const int64_t most = k.w == 16 ? 256 : 1024;
-  return (int)max((int64_t)1, min((rows + per - 1) / per, k.n == 0 ? min((int64_t)64, rows) : most / per));
+// Blocks of the backward pass's row walk.  Each leaves a share of 8 C bytes, so twice the CUs where rows are long (100000 x 1000
+// bf16: 114 us with 512 blocks, 134 with 1024; 24571 x 4096: 116 with 512, 131 with 256, 129 with 1024); narrow rows carry
+// little, and more blocks keep more loads on their way (50000 x 192: 24 us with 1024, 27 with 512).
+int backward_blocks(int64_t rows, int C, const Choice& k) {
+  if (k.n == 0) return (int)max((int64_t)1, min((int64_t)64, rows));
+  const int per = k.w >= 4 ? 1 : 4 / k.w;
+  const int64_t most = k.w == 16 ? 256 : C <= 256 ? 1024 : 512;
+  return (int)max((int64_t)1, min((rows + per - 1) / per, most));
 }
+// Entries of a row per thread: the backward pass holds five values for each, the forward pass one (20000 x 5120 fp16 forward: 97 us
+// on four waves with 32, 148 on sixteen with 16; 24571 x 4096 bf16: 92 on four waves, 96 on one with 64)
+constexpr int FORWARD = 32, BACKWARD = 16;
 
 template <class T, int VEC, int N, int W>
 void launch_one(const NormArgs& a, bool backward, hipStream_t s) {
   constexpr int R = W >= 4 ? 1 : 4 / W, threads = W > 4 ? 64 * W : 256;
-  if (backward) hipLaunchKernelGGL((norm_backward_kernel<T, VEC, N, W>), dim3(a.blocks / R), dim3(threads), 0, s, a);
-  else hipLaunchKernelGGL((norm_forward_kernel<T, VEC, N, W>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(threads), 0, s, a);
+  if (backward) {
+    if constexpr (N * VEC <= BACKWARD) hipLaunchKernelGGL((norm_backward_kernel<T, VEC, N, W>), dim3(a.blocks), dim3(threads), 0, s, a);
+  } else hipLaunchKernelGGL((norm_forward_kernel<T, VEC, N, W>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(threads), 0, s, a);
 }
 template <class T, int VEC, int N>
 void launch_w(const NormArgs& a, int w, bool backward, hipStream_t s) {
@@ -316,12 +376,13 @@ void launch_w(const NormArgs& a, int w, bool backward, hipStream_t s) {
 }
 template <class T, int VEC>
 void launch_n(const NormArgs& a, int n, int w, bool backward, hipStream_t s) {
-  constexpr int most = 16 / VEC;
+  constexpr int most = (FORWARD > BACKWARD ? FORWARD : BACKWARD) / VEC;
   if (n == 1) return launch_w<T, VEC, 1>(a, w, backward, s);
   if constexpr (most >= 2) { if (n == 2) return launch_w<T, VEC, 2>(a, w, backward, s); }
   if constexpr (most >= 4) { if (n == 4) return launch_w<T, VEC, 4>(a, w, backward, s); }
   if constexpr (most >= 8) { if (n == 8) return launch_w<T, VEC, 8>(a, w, backward, s); }
   if constexpr (most >= 16) { if (n == 16) return launch_w<T, VEC, 16>(a, w, backward, s); }
+  if constexpr (most >= 32) { if (n == 32) return launch_w<T, VEC, 32>(a, w, backward, s); }
 }
 template <class T>
 void launch(const NormArgs& a, const Choice& k, bool backward, hipStream_t s) {
@@ -333,7 +394,7 @@ void launch(const NormArgs& a, const Choice& k, bool backward, hipStream_t s) {
     }
   } else if (k.vec == 1) launch_n<T, 1>(a, k.n, k.w, backward, s);
   else launch_n<T, 16 / (int)sizeof(T)>(a, k.n, k.w, backward, s);
-  if (backward && a.part) hipLaunchKernelGGL((norm_join_kernel<T>), dim3((2 * a.C + 31) / 32), dim3(256), 0, s, a);
+  if (backward && a.part) hipLaunchKernelGGL((norm_join_kernel<T>), dim3((2 * a.C + 31) / 32), dim3(1024), 0, s, a);
 }
 
 int check(const ac_norm_args* p, const char* what) {
@@ -366,20 +427,18 @@ extern "C" int ac_layer_norm(const ac_norm_args* p, void* stream) {
   NormArgs a = {};
   a.x = p->x; a.y = p->y; a.w = p->weight; a.b = p->bias; a.x_row = p->x_row; a.y_row = p->y_row;
   a.mean = p->mean; a.rstd = p->rstd; a.rows = p->rows; a.C = p->width; a.w32 = p->weight_type == AC_F32; a.eps = p->eps;
-  const Choice k = choose(p->width, size, aligned16(p, {p->x, p->y}, {p->x_row, p->y_row}));
+  const Choice k = choose(p->width, size, aligned16(p, {p->x, p->y}, {p->x_row, p->y_row}), FORWARD);
   if (p->type == AC_F32) launch<float>(a, k, false, as_stream(stream));
   else if (p->type == AC_F16) launch<_Float16>(a, k, false, as_stream(stream));
   else launch<__bf16>(a, k, false, as_stream(stream));
   return ac_check_launch("ac_layer_norm");
 }
 
-// (the number of shares does not go by alignment: a workspace for the scalar kernels serves the others)
 static int norm_shares(const ac_norm_args* p, bool aligned) {
-  const Choice k = choose(p->width, p->type == AC_F32 ? 4 : 2, aligned);
-  const int per = k.n == 0 ? 1 : k.w >= 4 ? 1 : 4 / k.w;
-  return backward_blocks(p->rows, p->width, k) * per;
+  return backward_blocks(p->rows, p->width, choose(p->width, p->type == AC_F32 ? 4 : 2, aligned, BACKWARD));
 }
 
+// (a workspace for the one-entry kernels serves the 16-byte ones, and the other way round)
 extern "C" size_t ac_layer_norm_backward_workspace_bytes(const ac_norm_args* p) {
   if (check(p, "ac_layer_norm_backward") != AC_OK || p->rows == 0 || (!p->dweight && !p->dbias)) return 0;
   return (size_t)max(norm_shares(p, true), norm_shares(p, false)) * 2 * p->width * sizeof(float);
@@ -400,15 +459,15 @@ extern "C" int ac_layer_norm_backward(const ac_norm_args* p, void* ws, size_t ws
   AC_REQUIRE(((uintptr_t)ws & 3) == 0, "ac_layer_norm_backward: misaligned workspace");
   if (!p->dx && !p->dweight && !p->dbias) return AC_OK;
   const bool al = aligned16(p, {p->x, p->dy, p->dx}, {p->x_row, p->dy_row, p->dx_row});
-  const Choice k = choose(p->width, size, al);
+  const Choice k = choose(p->width, size, al, BACKWARD);
   a.blocks = norm_shares(p, al);
   a.part = need ? static_cast<float*>(ws) : nullptr;
   if (p->rows == 0) {                              // nothing to walk over: the sums are zero
     a.blocks = 0;
     if (p->dweight || p->dbias) {
-      if (p->type == AC_F32) hipLaunchKernelGGL((norm_join_kernel<float>), dim3((2 * a.C + 31) / 32), dim3(256), 0, as_stream(stream), a);
-      else if (p->type == AC_F16) hipLaunchKernelGGL((norm_join_kernel<_Float16>), dim3((2 * a.C + 31) / 32), dim3(256), 0, as_stream(stream), a);
-      else hipLaunchKernelGGL((norm_join_kernel<__bf16>), dim3((2 * a.C + 31) / 32), dim3(256), 0, as_stream(stream), a);
+      if (p->type == AC_F32) hipLaunchKernelGGL((norm_join_kernel<float>), dim3((2 * a.C + 31) / 32), dim3(1024), 0, as_stream(stream), a);
+      else if (p->type == AC_F16) hipLaunchKernelGGL((norm_join_kernel<_Float16>), dim3((2 * a.C + 31) / 32), dim3(1024), 0, as_stream(stream), a);
+      else hipLaunchKernelGGL((norm_join_kernel<__bf16>), dim3((2 * a.C + 31) / 32), dim3(1024), 0, as_stream(stream), a);
     }
     return ac_check_launch("ac_layer_norm_backward");
   }

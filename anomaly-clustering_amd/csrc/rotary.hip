@@ -7,7 +7,8 @@
 // so the factors are right to fp32 rounding at any position.  They are computed once per token and pair into LDS and used by
 // every head; products and sums are fp32, the result is rounded to the tensor's type once.
 //
-// Bound: each element is read once and written once; nothing else is of size.
+// Bound: memory; each element is read once and written once, nothing else is of size.  65536 tokens x 40 heads of 128 in bf16
+// (1.34 GB): 238 us, 5.6 TB/s, where a copy of 1 GB reaches 5.2.
 #include "common.h"
 
 namespace {
@@ -22,8 +23,6 @@ struct RotaryArgs {
   int dim, part, offset, axes, group;            // group: tokens per block
   float amplitude; int inverse;
 };
-
-template <class T> __device__ inline float to_f(T v) { return (float)v; }
 
 // cos and sin of a fp64 angle, to fp32
 __device__ inline void cos_sin(double x, float& c, float& s) {
@@ -49,26 +48,6 @@ __device__ inline void cos_sin(double x, float& c, float& s) {
 
 template <class T, int VEC> struct Pack { typedef T type __attribute__((ext_vector_type(VEC))); };
 template <class T> struct Pack<T, 1> { typedef T type; };
-template <class T, int VEC>
-__device__ inline void load(const T* p, float* v) {
-  typename Pack<T, VEC>::type x = *reinterpret_cast<const typename Pack<T, VEC>::type*>(p);
-  if constexpr (VEC == 1) v[0] = (float)x;
-  else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = (float)x[j];
-  }
-}
-template <class T, int VEC>
-__device__ inline void store(T* p, const float* v) {
-  typename Pack<T, VEC>::type x;
-  if constexpr (VEC == 1) x = (T)v[0];
-  else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) x[j] = (T)v[j];
-  }
-  *reinterpret_cast<typename Pack<T, VEC>::type*>(p) = x;
-}
-
 // One block: `group` tokens, all heads of q and k.  A unit is VEC elements of a head that pass, VEC neighbours that turn
 // (interleaved) or VEC pairs (half); thread -> (row, unit), a row being one head of one token.
 template <class T, int VEC, bool HALF>
@@ -93,49 +72,63 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   const int wide = min(units, 256), rows_at_once = 256 / wide;
   const int r0 = threadIdx.x / wide, u0 = threadIdx.x - r0 * wide;
   if (r0 >= rows_at_once) return;
-  const int heads = a.heads[0] + a.heads[1];
+  typedef typename Pack<T, VEC>::type raw;
+  const int heads = a.heads[0] + a.heads[1], rows = n * heads;
   for (int u = u0; u < units; u += wide) {
-    // an entry behind the turned ones passes: unit -> its place, skipping [offset, offset + part)
-    int at = HALF ? a.offset + u * VEC : a.offset + u * VEC;
-    const bool turns = u < turning;
-    if (!turns) {
-      at = (u - turning) * VEC;
-      if (at >= a.offset) at += a.part;
-    }
-    for (int row = r0; row < n * heads; row += rows_at_once) {
-      const int t = row / heads, hh = row - t * heads, which = hh >= a.heads[0], h = which ? hh - a.heads[0] : hh;
-      const T* src = static_cast<const T*>(a.src[which]) + (t0 + t) * a.s_tok[which] + h * a.s_head[which] + at;
-      T* dst = static_cast<T*>(a.dst[which]) + (t0 + t) * a.d_tok[which] + h * a.d_head[which] + at;
-      float x[VEC], y[VEC];
-      if (!turns) {
-        if (src != dst) {
-          load<T, VEC>(src, x);
-          store<T, VEC>(dst, x);
-        }
-      } else if constexpr (HALF) {
-        load<T, VEC>(src, x);
-        load<T, VEC>(src + pairs, y);
-        const float* c = cosines + t * pairs + u * VEC;
-        const float* s = sines + t * pairs + u * VEC;
-        float ox[VEC], oy[VEC];
+    // units in the order of their places (neighbouring lanes, neighbouring addresses); the half layout's skip the second entries
+    const int before = a.offset / VEC, turn = u - before;
+    const bool turns = turn >= 0 && turn < turning;
+    const int at = HALF && turn >= turning ? u * VEC + pairs : u * VEC;
+    // two rows at a time where a unit is two accesses, their loads first (65536 x 40 heads of 128: 238 us with two, 255 with four, 387
+    // with eight, which cost waves; interleaved, half of each head: 286 us with one, 308 with two)
+    constexpr int U = HALF ? 2 : 1;
+    for (int row = r0; row < rows; row += U * rows_at_once) {
+      raw x[U], y[U];
+      T* dst[U];
+      int tok[U];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          ox[j] = x[j] * c[j] - y[j] * s[j];
-          oy[j] = y[j] * c[j] + x[j] * s[j];
+      for (int j = 0; j < U; ++j) {
+        const int rj = row + j * rows_at_once;
+        const int t = rj / heads, hh = rj - t * heads, which = hh >= a.heads[0], h = which ? hh - a.heads[0] : hh;
+        tok[j] = rj < rows ? t : -1;
+        if (rj < rows) {
+          const T* src = static_cast<const T*>(a.src[which]) + (t0 + t) * a.s_tok[which] + h * a.s_head[which] + at;
+          dst[j] = static_cast<T*>(a.dst[which]) + (t0 + t) * a.d_tok[which] + h * a.d_head[which] + at;
+          x[j] = *reinterpret_cast<const raw*>(src);
+          if (HALF && turns) y[j] = *reinterpret_cast<const raw*>(src + pairs);
         }
-        store<T, VEC>(dst, ox);
-        store<T, VEC>(dst + pairs, oy);
-      } else if constexpr (VEC >= 2) {
-        load<T, VEC>(src, x);
-        const float* c = cosines + t * pairs + u * (VEC / 2);
-        const float* s = sines + t * pairs + u * (VEC / 2);
-        float o[VEC];
+      }
 #pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) {
-          o[2 * j] = x[2 * j] * c[j] - x[2 * j + 1] * s[j];
-          o[2 * j + 1] = x[2 * j + 1] * c[j] + x[2 * j] * s[j];
+      for (int j = 0; j < U; ++j) {
+        if (tok[j] < 0) continue;
+        raw* const out = reinterpret_cast<raw*>(dst[j]);
+        if (!turns) { *out = x[j]; continue; }
+        constexpr int P = HALF ? VEC : VEC / 2;    // pairs of a unit
+        const float* c = cosines + tok[j] * pairs + turn * P;
+        const float* s = sines + tok[j] * pairs + turn * P;
+        if constexpr (HALF) {
+          raw ox, oy;
+          if constexpr (VEC == 1) {
+            ox = (T)((float)x[j] * c[0] - (float)y[j] * s[0]);
+            oy = (T)((float)y[j] * c[0] + (float)x[j] * s[0]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              ox[i] = (T)((float)x[j][i] * c[i] - (float)y[j][i] * s[i]);
+              oy[i] = (T)((float)y[j][i] * c[i] + (float)x[j][i] * s[i]);
+            }
+          }
+          *out = ox;
+          *reinterpret_cast<raw*>(dst[j] + pairs) = oy;
+        } else if constexpr (VEC >= 2) {
+          raw o;
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            o[2 * i] = (T)((float)x[j][2 * i] * c[i] - (float)x[j][2 * i + 1] * s[i]);
+            o[2 * i + 1] = (T)((float)x[j][2 * i + 1] * c[i] + (float)x[j][2 * i] * s[i]);
+          }
+          *out = o;
         }
-        store<T, VEC>(dst, o);
       }
     }
   }
@@ -190,9 +183,10 @@ extern "C" int ac_rotary(const ac_rotary_args* r, void* stream) {
   a.positions = r->positions; a.pos_axis = r->position_axis; a.pos64 = r->positions64; a.freq = r->frequencies;
   a.tokens = r->tokens; a.dim = r->dim; a.part = r->part; a.offset = r->offset; a.axes = r->axes;
   a.amplitude = r->amplitude; a.inverse = r->inverse;
-  // tokens per block: about 2048 accesses for its 256 threads, fewer where that would leave CUs idle
+  // tokens per block: about 1024 accesses for its 256 threads (65536 tokens x 40 heads of 128, bf16, four rows at a time: 254 us with
+  // 1024 or 2048, 267 with 4096, 284 with 8192), fewer where that would leave CUs idle
   const int64_t per_token = (int64_t)(r->heads[0] + r->heads[1]) * (r->dim / vec);
-  int64_t group = max((int64_t)1, min((int64_t)16, 2048 / per_token));
+  int64_t group = max((int64_t)1, min((int64_t)16, 1024 / per_token));
   while (group > 1 && (r->tokens + group - 1) / group < 4 * ac_device_cus()) group /= 2;
   a.group = (int)group;
   const int64_t blocks = (r->tokens + group - 1) / group;
