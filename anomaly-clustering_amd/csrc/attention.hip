@@ -60,6 +60,39 @@ template <> struct Num<float> {
   }
 };
 
+// fp32 on the bf16 products: x = h + m + l, three bf16 values of 8 bits each, exactly (h and m cut off, no rounding, so that no
+// finite x overflows), and x y = h h + (h m + m h) + (m m + h l + l h), smallest first; what is left out is under 2^-21 of it.
+// Six products of 2.5 PFLOP/s peak against the 157 TFLOP/s of the fp32 instruction.  An infinity or NaN makes NaN, which the
+// end of the kernel looks for.
+struct Thirds { bf8 h, m, l; };
+__device__ inline Thirds thirds(const float (&x)[8]) {
+  u32x4 h, m, l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t a[2][3];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      a[i][0] = __builtin_bit_cast(uint32_t, x[2 * j + i]);
+      const float r = x[2 * j + i] - __builtin_bit_cast(float, a[i][0] & 0xffff0000u);
+      a[i][1] = __builtin_bit_cast(uint32_t, r);
+      const float q = r - __builtin_bit_cast(float, a[i][1] & 0xffff0000u);
+      a[i][2] = __builtin_bit_cast(uint32_t, q);
+    }
+    h[j] = __builtin_amdgcn_perm(a[1][0], a[0][0], 0x07060302u);       // the upper halves of two words
+    m[j] = __builtin_amdgcn_perm(a[1][1], a[0][1], 0x07060302u);
+    l[j] = __builtin_amdgcn_perm(a[1][2], a[0][2], 0x07060302u);
+  }
+  return {__builtin_bit_cast(bf8, h), __builtin_bit_cast(bf8, m), __builtin_bit_cast(bf8, l)};
+}
+__device__ inline f32x16 product(const Thirds& a, const Thirds& b, f32x16 c) {
+  c = Num<__bf16>::mfma(a.l, b.h, c);
+  c = Num<__bf16>::mfma(a.h, b.l, c);
+  c = Num<__bf16>::mfma(a.m, b.m, c);
+  c = Num<__bf16>::mfma(a.m, b.h, c);
+  c = Num<__bf16>::mfma(a.h, b.m, c);
+  return Num<__bf16>::mfma(a.h, b.h, c);
+}
+
 // ---- a tile of keys in LDS: rows of NS steps of 32 bytes (S = 2 NS slots of 16), slots moved by the row so that the reads
 // of neighbouring rows meet different banks: XOR where S is a power of two, rotation otherwise.
 template <int NS> struct Slots {
@@ -118,12 +151,15 @@ struct Shape {
   static constexpr int E = 16 / (int)sizeof(T);                            // entries of a slot
   static constexpr int DB = (NS * 2 * E + 31) / 32;                        // blocks of 32 entries of the output
   static constexpr int BUF = 2 * TILE;
+  static constexpr bool SPLIT = sizeof(T) == 4 && WQ > 1;                  // fp32 in thirds; few rows: the fp32 instruction
   static constexpr bool RING = sizeof(T) == 2 && WQ > 1 && 4 * BUF + 256 <= 160 * 1024;  // the pipelined loop: four tiles; else two
   static constexpr int BUFS = RING ? 4 : 2;
   static constexpr int JOIN = WK > 1 ? (WK - 1) * WQ * NQ * 64 * (DB * 16 + 2) * 4 : 0;
-  static constexpr int LDS = (BUFS * BUF + 256 > JOIN ? BUFS * BUF + 256 : JOIN);
+// SPLIT: V's three planes, K's, then the fp32 tile that they are made of
+  static constexpr int PLANE = TILE / 2, STAGE = 6 * PLANE;
+  static constexpr int LDS = SPLIT ? STAGE + BUF : BUFS * BUF + 256 > JOIN ? BUFS * BUF + 256 : JOIN;
   // registers: queries, output, two blocks of scores, weights, K and V fragments, the rest
-  static constexpr int REGS = NQ * (NS * 4 + DB * 16 + (RING ? 32 : 16) + (sizeof(T) == 2 ? 8 : 0)) + (RING ? 2 * NS * 4 : 16) + 40;
+  static constexpr int REGS = SPLIT ? NQ * (NS * 6 + DB * 16 + 40) + 56 : NQ * (NS * 4 + DB * 16 + (RING ? 32 : 16) + (sizeof(T) == 2 ? 8 : 0)) + (RING ? 2 * NS * 4 : 16) + 40;
   static constexpr int WAVES = REGS <= 128 && LDS <= 40960 ? 4 : REGS <= 168 && LDS <= 54000 ? 3 : REGS <= 256 && LDS <= 81920 ? 2 : 1;
   static constexpr int NI = TILE / 1024;                                   // transfers of 64 x 16 bytes per tile of K (or V)
   static constexpr int NJ = (NI + W - 1) / W;
@@ -256,7 +292,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
 #pragma unroll
   for (int j = 0; j < G::NJ; ++j) {
     const int chunk = (wave + G::W * j) * 64 + lane, row = chunk / S, place = chunk - row * S;
-    const int ks = L::slot_at(place, L::k_turn(row)), vs = L::slot_at(place, L::template v_turn<N::wide>(row));
+    const int ks = G::SPLIT ? place : L::slot_at(place, L::k_turn(row)), vs = G::SPLIT ? place : L::slot_at(place, L::template v_turn<N::wide>(row));
     koff[j] = ks * E < a.dim ? (uint32_t)row * ks_bytes + ks * 16 : 0x80000000u;      // behind the head: reads as zero
     voff[j] = vs * E < a.dim ? (uint32_t)row * vs_bytes + vs * 16 : 0x80000000u;
   }
@@ -270,7 +306,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
     const uint32_t kn = (uint32_t)(left - 1) * ks_bytes + a.dim * sizeof(T), vn = (uint32_t)(left - 1) * vs_bytes + a.dim * sizeof(T);
     const u32x4 kr = {first_lane((uint32_t)kb), first_lane((uint32_t)(kb >> 32)), first_lane(kn), 0x00020000u};
     const u32x4 vr = {first_lane((uint32_t)vb), first_lane((uint32_t)(vb >> 32)), first_lane(vn), 0x00020000u};
-    const uint32_t dst = lds_base + buffer * G::BUF;
+    const uint32_t dst = lds_base + (G::SPLIT ? G::STAGE : 0) + buffer * G::BUF;
 #pragma unroll
     for (int j = 0; j < G::NJ; ++j) {
       const int n = wave + G::W * j;
@@ -296,21 +332,34 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
     bool odd_values = false;                       // an infinity or NaN among values that not every row of the wave sees
     const int lim_least = active ? limit(wave_row) : 0, lim_most = active ? min(key_end, limit(min(wave_row + 32 * NQ, rows) - 1)) : 0;
     int lim[NQ];
-    frag qf[NQ][NS];
+    frag qf[G::SPLIT ? 1 : NQ][G::SPLIT ? 1 : NS];
+    Thirds qt[G::SPLIT ? NQ : 1][G::SPLIT ? NS / 2 : 1];
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
       const int row = wave_row + 32 * b + r, i = row / a.group, hh = kvh * a.group + row - i * a.group;
       lim[b] = row < rows ? limit(row) : 0;
       const T* src = static_cast<const T*>(a.q) + (int64_t)(q0 + i) * a.q_tok + (int64_t)hh * a.q_head;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const int d = (2 * s + h) * E;
+      auto words = [&](int d) {                    // 16 bytes of the row from entry d on
         frag z = {};
         u32x4 w = __builtin_bit_cast(u32x4, row < rows && d < a.dim ? *reinterpret_cast<const frag*>(src + d) : z);
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = (w[j] & a.q_keep) ^ a.q_flip;
-        if constexpr (G::WAVES == 1 && !N::wide) asm volatile("" : "+a"(w));       // in the accumulation registers, which the products read in place
-        qf[b][s] = __builtin_bit_cast(frag, w);
+        return w;
+      };
+      if constexpr (G::SPLIT) {
+#pragma unroll
+        for (int s = 0; s < NS / 2; ++s) {
+          const f32x4 lo = __builtin_bit_cast(f32x4, words(16 * s + 8 * h)), hi = __builtin_bit_cast(f32x4, words(16 * s + 8 * h + 4));
+          const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          qt[b][s] = thirds(x);
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          u32x4 w = words((2 * s + h) * E);
+          if constexpr (G::WAVES == 1 && !N::wide) asm volatile("" : "+a"(w));       // in the accumulation registers, which the products read in place
+          qf[b][s] = __builtin_bit_cast(frag, w);
+        }
       }
     }
     f32x16 o[NQ][DB];
@@ -330,17 +379,29 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
     // S^T of 32 keys, from LDS row `krow` of a tile on
     auto scores = [&](const uint8_t* Kt, int krow, f32x16 (&sc)[NQ]) {
       const uint8_t* krp = Kt + (krow + r) * P;
-      frag kf[NS];
-#pragma unroll
-      for (int s = 0; s < NS; ++s) kf[s] = *reinterpret_cast<const frag*>(krp + L::place(2 * s + h, kturn) * 16);
 #pragma unroll
       for (int b = 0; b < NQ; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[b][i] = 0.f;
+      if constexpr (G::SPLIT) {                    // Kt: K's planes
+        typedef Slots<NS / 2> H;
+        const int turn = H::k_turn(r);
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
+        for (int s = 0; s < NS / 2; ++s) {
+          const uint8_t* at = Kt + r * (P / 2) + H::place(2 * s + h, turn) * 16;
+          const Thirds k = {*reinterpret_cast<const bf8*>(at), *reinterpret_cast<const bf8*>(at + G::PLANE), *reinterpret_cast<const bf8*>(at + 2 * G::PLANE)};
 #pragma unroll
-        for (int b = 0; b < NQ; ++b) sc[b] = N::mfma(kf[s], qf[b][s], sc[b]);
+          for (int b = 0; b < NQ; ++b) sc[b] = product(k, qt[b][s], sc[b]);
+        }
+      } else {
+        frag kf[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) kf[s] = *reinterpret_cast<const frag*>(krp + L::place(2 * s + h, kturn) * 16);
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int b = 0; b < NQ; ++b) sc[b] = N::mfma(kf[s], qf[b][s], sc[b]);
+      }
     };
     // key: the block's first; some row of the wave does not see all of its keys
     auto mask = [&](const uint8_t* Vt, int krow, int key, f32x16 (&sc)[NQ]) {
@@ -350,10 +411,18 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
         for (int i = 0; i < 16; ++i) sc[b][i] = key + 8 * (i >> 2) + 4 * h + (i & 3) < lim[b] ? sc[b][i] : -__builtin_inff();
       // A masked score has p = 0, but 0 times an infinity or NaN is NaN: rows of a wave that meets one here are done again
       bool odd = false;
+      if constexpr (G::SPLIT) {                    // Vt: V's planes; the first shows them
 #pragma unroll
-      for (int j = 0; j < NS; ++j) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(Vt + krow * P + j * 1024 + lane * 16);
-        odd |= N::odd(w[0]) | N::odd(w[1]) | N::odd(w[2]) | N::odd(w[3]);
+        for (int j = 0; j < NS / 2; ++j) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(Vt + j * 1024 + lane * 16);
+          odd |= Num<__bf16>::odd(w[0]) | Num<__bf16>::odd(w[1]) | Num<__bf16>::odd(w[2]) | Num<__bf16>::odd(w[3]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(Vt + krow * P + j * 1024 + lane * 16);
+          odd |= N::odd(w[0]) | N::odd(w[1]) | N::odd(w[2]) | N::odd(w[3]);
+        }
       }
       if (__builtin_amdgcn_ballot_w64(odd)) odd_values = true;
       asm volatile("" ::: "memory");                   // (keeps this a branch: as selects it would cost every block)
@@ -406,11 +475,12 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
     // V^T fragments of 32 keys.  Transposed reads: lane 4 q + p of a 16-lane group addresses key row q, entries 4 p .. of the
     // group's 16, and gets column (lane & 15) of the 4 x 16 block; the groups take (entries 0 .. 15, 16 .. 31) x (lane halves)
     auto value_at = [&](const uint8_t* Vt, int krow, int d, int ks) {
+      typedef Slots<G::SPLIT ? NS / 2 : NS> H;
       u32x4 w;
 #pragma unroll
       for (int j2 = 0; j2 < 2; ++j2) {
         const int row = krow + 16 * ks + 8 * j2 + 4 * h + vq;
-        const uint8_t* at = Vt + row * P + L::place(4 * d + 2 * vg + (vp >> 1), L::template v_turn<false>(4 * h + vq)) * 16 + 8 * (vp & 1);
+        const uint8_t* at = Vt + row * H::P + H::place(4 * d + 2 * vg + (vp >> 1), H::template v_turn<false>(4 * h + vq)) * 16 + 8 * (vp & 1);
         const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at)));
         w[2 * j2] = x[0];
         w[2 * j2 + 1] = x[1];
@@ -419,6 +489,28 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
     };
     // O^T += V^T P^T
     auto values = [&](const uint8_t* Vt, int krow, const f32x16 (&sc)[NQ], const frag (&pf)[NQ][2]) {
+      if constexpr (G::SPLIT) {
+        Thirds pt[NQ][2];
+#pragma unroll
+        for (int b = 0; b < NQ; ++b)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = sc[b][8 * ks + i];
+            pt[b][ks] = thirds(x);
+          }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const Thirds v = {__builtin_bit_cast(bf8, value_at(Vt, 0, d, ks)), __builtin_bit_cast(bf8, value_at(Vt + G::PLANE, 0, d, ks)),
+                              __builtin_bit_cast(bf8, value_at(Vt + 2 * G::PLANE, 0, d, ks))};
+#pragma unroll
+            for (int b = 0; b < NQ; ++b) o[b][d] = product(v, pt[b][ks], o[b][d]);
+          }
+        return;
+      }
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
         if constexpr (N::wide) {
@@ -503,6 +595,44 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
         step(j, sa, sb);
         if (j + 1 < blocks) step(j + 1, sb, sa);
       }
+    } else if constexpr (G::SPLIT) {
+      // A tile of 32 keys arrives in fp32; each thread cuts its share of it into thirds once for the whole block, and the next tile
+      // is on its way while this one's planes are multiplied (each wave cutting every tile for itself: 402 us instead of MEASURED
+      // for 32 images of 785 tokens).
+      static_assert(KB == 1 && WK == 1, "");
+      typedef Slots<NS / 2> H;
+      if (tiles) fetch(split_begin, 0);
+      for (int t = 0; t < tiles; ++t) {
+        wait_transfers<0>();
+        barrier();                                 // the tile is there; the planes of the last one are read
+#pragma unroll
+        for (int c = tid; c < 64 * NS; c += G::THREADS) {
+          const bool value = c < 32 * NS;
+          const int at = value ? c : c - 32 * NS, row = at / NS, slot = at - row * NS;
+          const uint8_t* from = lds + G::STAGE + (value ? G::TILE : 0) + row * P + slot * 32;
+          const f32x4 lo = *reinterpret_cast<const f32x4*>(from), hi = *reinterpret_cast<const f32x4*>(from + 16);
+          const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          const Thirds y = thirds(x);
+          uint8_t* to = lds + (value ? 0 : 3 * G::PLANE) + row * (P / 2) + H::place(slot, value ? H::template v_turn<false>(row) : H::k_turn(row)) * 16;
+          *reinterpret_cast<bf8*>(to) = y.h;
+          *reinterpret_cast<bf8*>(to + G::PLANE) = y.m;
+          *reinterpret_cast<bf8*>(to + 2 * G::PLANE) = y.l;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        barrier();
+        if (t + 1 < tiles) fetch(split_begin + (t + 1) * G::KEYS, 0);
+        const int key = split_begin + t * G::KEYS;
+        if (key >= lim_most) continue;
+        f32x16 sc[NQ];
+        frag pf[NQ][2];
+        float top[NQ];
+        scores(lds + 3 * G::PLANE, 0, sc);
+        if (key + 32 > lim_least) mask(lds, 0, key, sc);
+        maxima(sc, top);
+        rescale(top);
+        weights(sc, pf);
+        values(lds, 0, sc, pf);
+      }
     } else {
       if (tiles) fetch(split_begin, 0);
       for (int t = 0; t < tiles; ++t) {
@@ -562,6 +692,18 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
             m_run[b] = m_new;
           }
       }
+    }
+    if constexpr (G::SPLIT) {                      // NaN: there may be an infinity behind it, which the thirds cannot hold
+      bool nan = false;
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
+        nan |= l_run[b] != l_run[b];
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) nan |= o[b][d][i] != o[b][d][i];
+      }
+      if (__builtin_amdgcn_ballot_w64(nan)) odd_values = true;
     }
     if constexpr (WK > 1) {
       __syncthreads();
@@ -740,7 +882,7 @@ int launch_kind(const AttArgs& a, int kind, hipStream_t stream) {
     else return launch<T, NS, 1, 1, Num<T>::wide ? 4 : 2, 1>(a, stream);
   }
   if constexpr (NS * 32 > 512) return launch<T, NS, 1, 4, 1, 1>(a, stream);
-  else return launch<T, NS, 1, 4, 1, big ? 1 : 2>(a, stream);
+  else return launch<T, NS, 1, 4, 1, big || Num<T>::wide ? 1 : 2>(a, stream);
 }
 
 template <class T>
