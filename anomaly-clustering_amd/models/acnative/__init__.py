@@ -1076,8 +1076,8 @@ def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, c
     q [tokens, heads, dim], k and v [key tokens, kv_heads, dim], heads a multiple of kv_heads; float32, float16 or bfloat16;
     dim a multiple of 8 up to 256.  Sequence s is the rows starts_q[s] .. starts_q[s + 1] of q and starts_k[s] .. of k and v
     (int32 [sequences + 1] on the device; sequence_starts makes them); starts_k=None: the same as starts_q.  max_q / max_k: upper
-    bounds of the lengths - they shape the launch and never the result; None takes the number of tokens.  causal: query i of n
-    sees key j of m where j <= i + m - n.  A row that sees no key is zero; rows outside every sequence are left as they
+    bounds of the lengths - they shape the launch and never which rows are computed; None takes the number of tokens.  causal:
+    query i of n sees key j of m where j <= i + m - n.  A row that sees no key, or none with a score above -inf, is zero; rows outside every sequence are left as they
     were in `out` (without `out`: zero).  scale: 1 / sqrt(dim) unless given.  want_sums: also the fp32 [tokens, heads] logarithm of
     each row's sum of exponentials (-inf for a row that sees no key, and outside every sequence).
     Tensors whose heads do not start at multiples of 16 bytes are copied first."""
@@ -1134,7 +1134,7 @@ def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, c
         ks, vs = (0, ks[1]), (0, vs[1])
     args = _pack_attention(qp, kp, vp, out.data_ptr(), sums.data_ptr() if want_sums else 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
                            starts_q.data_ptr(), starts_k.data_ptr(), tokens, keys, sequences, heads, kv_heads, dim,
-                           tokens if max_q is None else max_q, keys if max_k is None else max_k, bool(causal), clear + 2 * want_sums,
+                           tokens if max_q is None else min(max_q, tokens), keys if max_k is None else min(max_k, keys), bool(causal), clear + 2 * want_sums,
                            _TYPES[dtype], dim ** -0.5 if scale is None else scale)
     handle = lib()
     n = handle.ac_attention_packed_workspace_bytes(args)

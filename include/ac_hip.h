@@ -357,10 +357,10 @@ int ac_rotary(const ac_rotary_args* args, void* stream);
 
 /* Attention over packed sequences: out[t, h] = sum_j p_j v[j, g], p = softmax(scale * q[t, h] . k[j, g]) over the keys of the
  * token's own sequence, g = h / (heads / kv_heads).  causal: query i of n sees key j of m where j <= i + m - n (the last query
- * sees every key).  A row that sees no key is zero and its log-sum -inf; a key that a row does not see cannot touch it,
- * whatever it holds.  Rows before the first and behind the last sequence are left as they are; clear
+ * sees every key).  A row that sees no key (or none with a score above -inf) is zero and its log-sum -inf; a key that a
+ * row does not see cannot touch it, whatever it holds.  Rows before the first and behind the last sequence are left as they are; clear
  * & 1 makes them zero in out, clear & 2 -inf in sums.
- * starts_q, starts_k: int32 [sequences + 1] on the device, clamped there to 0 .. tokens.  max_q, max_k: upper bounds of the
+ * starts_q, starts_k: int32 [sequences + 1] on the device, not decreasing, clamped there to 0 .. tokens.  max_q, max_k: upper bounds of the
  * lengths, used for the launch's shape alone (too small a bound costs time, not rows).  sums (nullable): fp32 [tokens_q,
  * heads], the natural logarithm of each row's sum of exponentials.  out must not overlap q, k or v. */
 typedef struct ac_attention_args {

@@ -365,3 +365,141 @@ def test_images_of_their_own_sizes_as_a_backbone_would(dev):
     ref = opacked.attention(rq, rk, qkv[:, 2 * H:], starts.cpu(), starts.cpu(), False)
     ref["score"] = ref["score"] * (1 + 2.0 ** -20 / E / (2 * D + 6))          # the turned q and k are off by 2^-21 each
     _check_attention(got, sums, ref, "fp32", D, "chain")
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("lengths", [([200, 30], None), ([1, 2], [300, 700])])
+def test_attention_with_infinite_keys_and_values(dev, kind, lengths):
+    """What rows do see: a key whose scores are -inf is left out, one at +inf makes NaN, infinite values pass where they weigh."""
+    queries, keys = lengths
+    sq, sk = _starts(queries), _starts(keys or queries)
+    H, D = 2, 64
+    q = _randn((int(sq[-1]), H, D), 1, kind).abs() + 0.125                  # positive: the sign of an infinite key decides
+    k, v = _randn((int(sk[-1]), H, D), 2, kind), _randn((int(sk[-1]), H, D), 3, kind)
+    k[5, 0, 3] = -math.inf
+    v[9, 1, 4] = math.inf
+    v[10, 1, 5] = math.nan
+    ref = opacked.attention(q, torch.where(torch.isinf(k), torch.zeros_like(k), k), v, sq, sk, False)
+    # without key 5 for head 0 of the first sequence
+    keep = torch.ones(int(sk[-1]), dtype=torch.bool)
+    keep[5] = False
+    lens = [n for n in (keys or queries)]
+    lens[0] -= 1
+    less = opacked.attention(q, k[keep], v[keep], sq, _starts(lens), False)
+    first = slice(0, queries[0])
+    for key in ref:
+        ref[key][first, 0] = less[key][first, 0]
+    args = [t.to(dev) for t in (q, k, v, sq, sk)]
+    got, sums = acnative.attention_packed(*args, want_sums=True)
+    _check_attention(got, sums, ref, kind, D, "infinite")
+    k[7, 0, 1] = math.inf
+    got = acnative.attention_packed(args[0], k.to(dev), *args[2:]).cpu()
+    assert torch.isnan(got[first, 0]).all() and torch.equal(got[first, 1].isnan(), ref["out"][first, 1].isnan())
+    assert torch.isfinite(got[queries[0]:]).all()
+    k[:] = -math.inf                                                         # no score above -inf: zero
+    got, sums = acnative.attention_packed(args[0], k.to(dev), torch.nan_to_num(v).to(dev), *args[3:], want_sums=True)
+    assert (got == 0).all() and (sums == -math.inf).all()
+
+
+def test_attention_large_and_small_magnitudes_in_fp32(dev):
+    """fp32 in thirds: values near the largest float and far under 1 keep their digits."""
+    sq = _starts([90, 40])
+    for scale in (1e30, 1e-30):
+        q, k, v = _randn((130, 2, 64), 1, "fp32"), _randn((130, 2, 64), 2, "fp32"), _randn((130, 2, 64), 3, "fp32") * scale
+        ref = opacked.attention(q, k, v, sq, sq, True)
+        got = acnative.attention_packed(q.to(dev), k.to(dev), v.to(dev), sq.to(dev), causal=True)
+        err = (got.cpu().double() - ref["out"]).abs()
+        assert (err <= _u("fp32") * ref["out"].abs() + (2 * (2 * 64 + 6) * E * ref["score"] + (ref["keys"] + 8) * E)[..., None] * ref["weighted"]).all()
+        q2, k2 = q * 1e15, k * 1e-15
+        got = acnative.attention_packed(q2.to(dev), k2.to(dev), q.to(dev), sq.to(dev), causal=True)
+        ref2 = opacked.attention(q2, k2, q, sq, sq, True)
+        err = (got.cpu().double() - ref2["out"]).abs()
+        assert (err <= _u("fp32") * ref2["out"].abs() + (2 * (2 * 64 + 6) * E * ref2["score"] + (ref2["keys"] + 8) * E)[..., None] * ref2["weighted"]).all()
+
+
+def test_attention_many_sequences(dev):
+    """More than 64 sequences (not ordered by length), and a thousand short ones."""
+    g = torch.Generator().manual_seed(4)
+    for count, top in ((65, 200), (1000, 9)):
+        n = torch.randint(0, top, (count,), generator=g).tolist()
+        _run(dev, "bf16", 4, 2, 64, n, causal=True, seed=count)
+        _run(dev, "fp16", 2, 2, 32, [1] * count, [x + 1 for x in n], causal=True, seed=count + 1)
+
+
+def test_attention_both_calls_at_once(dev):
+    """Two streams at a time, each with its own split key axis: the same as one after the other."""
+    sq, sk = _starts([1, 1]).to(dev), _starts([6000, 5000]).to(dev)
+    sets = [[_randn((2, 8, 128), i, "bf16").to(dev), _randn((11000, 2, 128), i + 1, "bf16").to(dev), _randn((11000, 2, 128), i + 2, "bf16").to(dev)] for i in (1, 11)]
+    alone = [acnative.attention_packed(*s, sq, sk, max_q=1, max_k=6000, causal=True) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        got = []
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(acnative.attention_packed(*s, sq, sk, max_q=1, max_k=6000, causal=True))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(alone, got))
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_the_attention_half_of_a_block(dev, kind):
+    """Norm, projection, rotary positions, attention over images of their own sizes; then the norm's gradients from the projection's:
+    each step against float64 on the step's own input."""
+    grids, H, G, D = [(3, 5), (12, 12), (1, 1), (7, 20)], 6, 2, 32
+    C = H * D
+    lengths = [a * b + 1 for a, b in grids]
+    T = sum(lengths)
+    pos = torch.cat([torch.cat([torch.zeros(2, 1, dtype=torch.int64), torch.stack([torch.arange(a * b) // b, torch.arange(a * b) % b])], 1) for a, b in grids], 1)
+    starts, longest = acnative.sequence_starts(lengths, dev)
+    x, dy = _randn((T, C), 1, kind).to(dev), _randn((T, C), 2, kind).to(dev)
+    w, b = (1 + 0.2 * _randn((C,), 3, "fp32")).to(dev), _randn((C,), 4, "fp32").to(dev)
+    proj = (_randn(((H + 2 * G) * D, C), 5, "fp32") / C ** 0.5).to(KINDS[kind]).to(dev)
+    freq = acnative.rotary_frequencies(D, 100.0, axes=2, device=dev)
+    y, mean, rstd = acnative.layer_norm(x, w, b, want_stats=True)
+    xd = x.cpu().double().requires_grad_()
+    wd = w.cpu().double().requires_grad_()
+    bd = b.cpu().double().requires_grad_()
+    yd = torch.nn.functional.layer_norm(xd, (C,), wd, bd, 1e-6)
+    assert ((y.cpu().double() - yd).abs() <= _u(kind) * yd.abs() + 1e-5).all()
+    qkv = (y.float() @ proj.float().T).to(KINDS[kind]).view(T, H + 2 * G, D)
+    q, k, v = qkv[:, :H], qkv[:, H:H + G], qkv[:, H + G:]
+    rq, sq_ = opacked.rotary(q.cpu(), pos, freq.cpu(), "half", 0, 1.0)
+    acnative.rotary(q, k, pos.to(dev), freq, out_q=q, out_k=k)
+    assert ((q.cpu().double() - rq).abs() <= _u(kind) * rq.abs() + (2.0 ** -22 + 4 * E) * sq_).all()
+    got, sums = acnative.attention_packed(q, k, v, starts, max_q=longest, max_k=longest, want_sums=True)
+    ref = opacked.attention(q.cpu(), k.cpu(), v.cpu(), starts.cpu(), starts.cpu(), False)
+    _check_attention(got, sums, ref, kind, D, "half block")
+    dx, dw, db = acnative.layer_norm_backward(dy, x, w, mean, rstd)
+    gx, gw, gb = torch.autograd.grad(yd, (xd, wd, bd), dy.cpu().double())
+    assert ((dx.cpu().double() - gx).abs() <= _u(kind) * gx.abs() + 2e-5 * gx.abs().max()).all()
+    assert ((dw.cpu().double() - gw).abs() <= 1e-5 * (1 + gw.abs().max())).all() and ((db.cpu().double() - gb).abs() <= 1e-5 * (1 + gb.abs().max())).all()
+
+
+def test_wrappers_refuse_what_they_say(dev):
+    x = torch.zeros(8, 4, 64, device=dev)
+    starts = torch.tensor([0, 8], dtype=torch.int32, device=dev)
+    freq = acnative.rotary_frequencies(64, device=dev)
+    pos = torch.zeros(8, dtype=torch.int32, device=dev)
+    a = acnative.attention_packed
+    for error, call in (
+            (TypeError, lambda: a(x, x.half(), x, starts)), (TypeError, lambda: a(x.double(), x.double(), x.double(), starts)),
+            (ValueError, lambda: a(x, x[:, :, :32], x[:, :, :32], starts)), (ValueError, lambda: a(x, x[:, :2], x, starts)),
+            (RuntimeError, lambda: a(x, x[:, :3], x[:, :3], starts)), (TypeError, lambda: a(x, x, x, starts.long())),
+            (RuntimeError, lambda: a(x, x, x, starts.cpu())), (ValueError, lambda: a(x, x[:4], x[:4], starts)),
+            (ValueError, lambda: a(x, x, x, starts, starts[:1])), (ValueError, lambda: a(x[0], x[0], x[0], starts)),
+            (ValueError, lambda: a(x, x, x, starts, out=x)), (ValueError, lambda: a(x, x, x, starts, out=x.new_zeros(8, 4, 32).repeat(1, 1, 2)[:, :2])),
+            (ValueError, lambda: a(x, x, x, starts, out=x.new_zeros(8, 1, 64).expand(8, 4, 64))), (RuntimeError, lambda: a(x, x, x, starts, scale=math.inf)),
+            (ValueError, lambda: a(x.transpose(1, 2), x.transpose(1, 2), x.transpose(1, 2), starts)),
+            (RuntimeError, lambda: a(x.clone().requires_grad_(), x, x, starts)),
+            (ValueError, lambda: acnative.rotary(x, None, pos, freq, layout="other")), (TypeError, lambda: acnative.rotary(x, None, pos.float(), freq)),
+            (TypeError, lambda: acnative.rotary(x, None, pos, freq.float())), (ValueError, lambda: acnative.rotary(x, None, pos[:4], freq)),
+            (RuntimeError, lambda: acnative.rotary(x, None, pos, freq, offset=2)), (ValueError, lambda: acnative.rotary(x, x[:4], pos, freq)),
+            (ValueError, lambda: acnative.rotary(x, None, pos, freq, out_k=x)), (ValueError, lambda: acnative.rotary(x[:, :2], x[:, 2:], pos, freq, out_q=x[:, 1:3])),
+            (ValueError, lambda: acnative.layer_norm(x, torch.ones(32, device=dev))), (TypeError, lambda: acnative.layer_norm(x, torch.ones(64, device=dev).half())),
+            (ValueError, lambda: acnative.layer_norm(x[:4], out=x[1:5])), (RuntimeError, lambda: acnative.layer_norm(x.clone().requires_grad_())),
+            (ValueError, lambda: acnative.layer_norm_backward(x[:2], x, None, x[:, :, 0].contiguous(), x[:, :, 0].contiguous())),
+            (ValueError, lambda: acnative.layer_norm_backward(x, x, None, pos.float(), pos.float()))):
+        with pytest.raises(error):
+            call()
+    assert acnative.attention_packed(x, x, x, starts, max_q=10 ** 12, max_k=10 ** 12).shape == x.shape
