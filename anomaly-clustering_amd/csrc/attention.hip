@@ -8,13 +8,21 @@
 //
 // A row is one query of one head; the rows of a key head's group are taken together (row r = query r / group, head
 // r % group), so K and V are read once for the group and a single query still fills `group` rows.
+//
+// Bounds, and what was reached (16-bit heads unless said otherwise; a large matrix product reaches 1390 TFLOP/s here):
+//   many rows: the products and the exponentials, which share a wave's issue.  A 32x32x16 product takes 32 clocks of the matrix
+//     unit; beside it one wave hides 4 vector instructions, two waves of a SIMD 6.  Heads of 128 (64 rows a wave, one wave a SIMD,
+//     its loop pipelined): 1040 TFLOP/s on a causal prompt of 16384; heads of 64 (two waves a SIMD), where a score has half the
+//     products to its exponential: 920 on 4096 x 4096; images of 1 .. 2305 tokens 630, of which a quarter is rows that do not
+//     fill a tile.  64 rows a wave, because K and V come from LDS: with 32 the reads alone would take as long as the products.
+//   single queries: the bytes of K and V.  64 on 4096 keys each 5.9 TB/s, 16 on 1 .. 16000 keys 4.8 (a copy: 5.2).
+//   fp32: six bf16 products for one (below), 176 .. 204 TFLOP/s, where the fp32 instruction reached 105 .. 140.
 #include "common.h"
 
 namespace {
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -155,7 +163,7 @@ struct Shape {
   static constexpr bool RING = sizeof(T) == 2 && WQ > 1 && 4 * BUF + 256 <= 160 * 1024;  // the pipelined loop: four tiles; else two
   static constexpr int BUFS = RING ? 4 : 2;
   static constexpr int JOIN = WK > 1 ? (WK - 1) * WQ * NQ * 64 * (DB * 16 + 2) * 4 : 0;
-// SPLIT: V's three planes, K's, then the fp32 tile that they are made of
+  // SPLIT: V's three planes, K's, then the fp32 tile that they are made of
   static constexpr int PLANE = TILE / 2, STAGE = 6 * PLANE;
   static constexpr int LDS = SPLIT ? STAGE + BUF : BUFS * BUF + 256 > JOIN ? BUFS * BUF + 256 : JOIN;
   // registers: queries, output, two blocks of scores, weights, K and V fragments, the rest
@@ -763,7 +771,8 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
 // more, up to 256).  The parts' maxima and sums: lane -> part.
 template <class T>
 __global__ __launch_bounds__(256) void join_kernel(const AttArgs a) {
-  __shared__ float weight[64], all[8][260];
+  __shared__ float weight[64];
+  __shared__ __attribute__((aligned(16))) float all[8][260];
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const int token = (int)(row / a.heads), hh = (int)(row - (int64_t)token * a.heads);

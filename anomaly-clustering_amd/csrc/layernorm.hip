@@ -7,7 +7,8 @@
 //
 // Bound: memory.  A row lives in the registers of the wave or block that owns it, so x (and dy) are read once; a block of the
 // backward pass walks over many rows with its share of dw and db in registers, and a second kernel adds the blocks' shares
-// in a fixed order (no atomics: the same bits every time).
+// in a fixed order (no atomics: the same bits every time).  24571 x 4096 bf16: forward 92 us (4.4 TB/s), backward with its sums
+// 116 us (5.2 TB/s); 25120 x 768 fp32: 26 and 43 us (a copy of that size stays in the cache: 6 .. 8 TB/s).
 #include <initializer_list>
 
 #include "common.h"
