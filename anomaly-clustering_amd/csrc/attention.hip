@@ -459,6 +459,8 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
           m_run[b] = m_new;
         }
     };
+    // Weights: fp32 in the sum; rounded to the tensor's type (16-bit) for the product with the values, as the matrix instructions
+    // take them: half a step, 2^-9 or 2^-12 relative, of each weight, next to the same of the result
     auto weights = [&](f32x16 (&sc)[NQ], frag (&pf)[NQ][2]) {
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {

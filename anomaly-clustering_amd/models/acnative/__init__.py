@@ -896,6 +896,11 @@ except ImportError:
         return torch.cuda.current_stream(index).cuda_stream
 
 
+def _fresh(t):
+    """An uninitialised contiguous tensor of t's shape and type."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _no_cpu(t, name):
     raise RuntimeError("%s must be a tensor on the HIP device (got %s); the MI355X path has no CPU fallback" % (name, getattr(t, "device", type(t))))
 
@@ -1038,14 +1043,14 @@ def rotary(q, k, positions, frequencies, layout="half", offset=0, amplitude=1.0,
     if pshape != (axes, tokens) and not (axes == 1 and pshape == (tokens,)):
         raise ValueError("positions must be [%d, %d]%s, got %s" % (axes, tokens, " or [%d]" % tokens if axes == 1 else "", tuple(pshape)))
     if out_q is None:
-        out_q = q.new_empty(shape)
+        out_q = _fresh(q)
         os = (heads * dim, dim)
     else:
         os = _rotary_out(out_q, "out_q", q, like, q, k)
     kos = (0, 0)
     if k is not None:
         if out_k is None:
-            out_k = k.new_empty(kshape)
+            out_k = _fresh(k)
             kos = (kv_heads * dim, dim)
         else:
             kos = _rotary_out(out_k, "out_k", k, like, q, k)
@@ -1105,7 +1110,7 @@ def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, c
     sequences = count[0] - 1
     clear = out is None
     if clear:
-        out = q.new_empty(shape)
+        out = _fresh(q)
         os = (heads * dim, dim)
     else:
         _, os = _heads(out, "out", like)
@@ -1203,7 +1208,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, want_stats=False):
         if bias is not None and bias.dtype != kind:
             raise TypeError("weight is %s, but bias is %s" % (kind, bias.dtype))
     if out is None:
-        out = x.new_empty(x.shape)
+        out = _fresh(x)
         out_row, to = width, out
     else:
         to = _rows(out, "out", x)
@@ -1238,9 +1243,11 @@ def layer_norm_backward(dy, x, weight, mean, rstd, want=(True, True, True)):
         _whole(t, (torch.float32,), name, device)
         if t.shape != x.shape[:-1]:
             raise ValueError("%s must be %s, got %s" % (name, tuple(x.shape[:-1]), tuple(t.shape)))
-    dx = x.new_empty(x.shape) if want[0] else None
-    dw = x.new_empty(width, dtype=kind) if want[1] else None
-    db = x.new_empty(width, dtype=kind) if want[2] else None
+    dx = _fresh(x) if want[0] else None
+    if weight is None:
+        dw, db = (x.new_empty(width, dtype=kind) if w else None for w in want[1:])
+    else:
+        dw, db = (_fresh(weight) if w else None for w in want[1:])
     args = _pack_norm(rows.data_ptr(), 0 if weight is None else weight.data_ptr(), 0, 0, grads.data_ptr(), 0 if dx is None else dx.data_ptr(),
                       0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
                       rows.stride(0) if count > 1 else width, 0, grads.stride(0) if count > 1 else width, width, count, width, _TYPES[dtype], _TYPES[kind], 0.0)
