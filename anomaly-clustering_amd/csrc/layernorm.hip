@@ -7,8 +7,8 @@
 //
 // Bound: memory.  A row lives in the registers of the wave or block that owns it, so x (and dy) are read once; a block of the
 // backward pass walks over many rows with its share of dw and db in registers, and a second kernel adds the blocks' shares
-// in a fixed order (no atomics: the same bits every time).  24571 x 4096 bf16: forward 92 us (4.4 TB/s), backward with its sums
-// 116 us (5.2 TB/s); 25120 x 768 fp32: 26 and 43 us (a copy of that size stays in the cache: 6 .. 8 TB/s).
+// in a fixed order (no atomics: the same bits every time).  24571 x 4096 bf16: forward 88 us (4.6 TB/s), backward with its sums
+// 115 us (5.2 TB/s); 25120 x 768 fp32: 26 and 43 us (a copy of that size stays in the cache: 6 .. 8 TB/s).
 #include <initializer_list>
 
 #include "common.h"
@@ -55,11 +55,19 @@ __device__ inline void load_w(const void* p, int w32, int at, float* v) {
   } else load<T, VEC>(static_cast<const T*>(p) + at, v);
 }
 
-// sum over the W waves that share a row: [2] values
-template <int W>
+// sums of two values over the L lanes of each of the W waves that share a row (L < 64: several rows to a wave)
+template <int W, int L = 64>
 __device__ inline void row_sum(float& a, float& b, float (*box)[2], int wave) {
-  a = wave_sum(a);
-  b = wave_sum(b);
+  if constexpr (L == 64) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+  } else {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+      a += __shfl_xor(a, o, 64);
+      b += __shfl_xor(b, o, 64);
+    }
+  }
   if constexpr (W > 1) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) { box[wave][0] = a; box[wave][1] = b; }
@@ -70,30 +78,31 @@ __device__ inline void row_sum(float& a, float& b, float (*box)[2], int wave) {
   }
 }
 
-// N chunks of VEC entries per thread, W waves per row; 4 / W rows (at least one) per block.  One row per wave or block: a walk over
+// N chunks of VEC entries per thread, W waves per row or L lanes (narrow rows); as many rows per block as its 256 threads hold.  One row per wave or block: a walk over
 // several with the next one's loads ahead, as the backward pass does it, was slower (24571 x 4096 bf16: 86 us, 92 .. 100 walking).
-template <class T, int VEC, int N, int W>
-__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_forward_kernel(const NormArgs a) {
-  constexpr int R = W >= 4 ? 1 : 4 / W;
+// (five waves a SIMD at least: left to itself hipcc may fetch all weights at once into 210 registers - 8000 x 8192 fp32: 194 us, 101 so)
+template <class T, int VEC, int N, int W, int L>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256, W > 4 ? 4 : 5) void norm_forward_kernel(const NormArgs a) {
+  constexpr int R = W >= 4 ? 1 : 256 / L, THREADS = L * W;       // rows per block, threads per row
   typedef typename Pack<T, VEC>::type raw;
   __shared__ float box[W][2];
-  const int tid = threadIdx.x, wave = tid >> 6, t = R == 1 ? tid : tid % (64 * W);
+  const int tid = threadIdx.x, wave = tid >> 6, t = R == 1 ? tid : tid % THREADS;
   const int chunks = a.C / VEC;
-  const int64_t row = (int64_t)blockIdx.x * R + (R == 1 ? 0 : wave / W);
-  if (row >= a.rows) return;                      // (whole waves; R > 1 only with W == 1, where no barrier follows)
+  const int64_t row = (int64_t)blockIdx.x * R + (R == 1 ? 0 : tid / THREADS);
+  if (row >= a.rows) return;                      // (all the lanes that a sum is taken over; R > 1 only with W == 1, where no barrier follows)
   {
     const T* from = static_cast<const T*>(a.x) + row * a.x_row;
     raw x[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = t + 64 * W * i;
+      const int c = t + THREADS * i;
       if (c < chunks) x[i] = *reinterpret_cast<const raw*>(from + c * VEC);
     }
     float v[N][VEC];
     float s = 0.f, zero = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (t + 64 * W * i < chunks) {
+      if (t + THREADS * i < chunks) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           if constexpr (VEC == 1) v[i][j] = (float)x[i];
@@ -102,22 +111,22 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_forward_kernel(cons
         }
       }
     }
-    row_sum<W>(s, zero, box, wave);
+    row_sum<W, L>(s, zero, box, wave);
     const float mean = s / (float)a.C;
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (t + 64 * W * i < chunks) {
+      if (t + THREADS * i < chunks) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) { v[i][j] -= mean; q += v[i][j] * v[i][j]; }
       }
     }
-    row_sum<W>(q, zero, box, wave);
+    row_sum<W, L>(q, zero, box, wave);
     const float rstd = 1.0f / sqrtf(q / (float)a.C + a.eps);
     T* y = static_cast<T*>(a.y) + row * a.y_row;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = t + 64 * W * i;
+      const int c = t + THREADS * i;
       if (c < chunks) {
         float w[VEC], b[VEC], o[VEC];
         if (a.w) load_w<T, VEC>(a.w, a.w32, c * VEC, w);
@@ -137,18 +146,18 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_forward_kernel(cons
 
 // The next row's loads are issued before this row's sums are taken, so that a block always has two rows on their way (one row at
 // a time: 133 us for 24571 x 4096 bf16, 4.5 TB/s).
-template <class T, int VEC, int N, int W>
+template <class T, int VEC, int N, int W, int L>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_backward_kernel(const NormArgs a) {
-  constexpr int R = W >= 4 ? 1 : 4 / W;           // rows in flight per block
+  constexpr int R = W >= 4 ? 1 : 256 / L, THREADS = L * W;       // rows in flight per block, threads per row
   typedef typename Pack<T, VEC>::type raw;
   __shared__ float box[W][2];
-  __shared__ float share[R > 1 ? 2 * 64 * N * VEC : 1];
-  const int tid = threadIdx.x, wave = tid >> 6, t = R == 1 ? tid : tid % (64 * W), sub = R == 1 ? 0 : wave / W;
+  __shared__ float share[R > 1 ? 2 * L * N * VEC : 1];
+  const int tid = threadIdx.x, wave = tid >> 6, t = R == 1 ? tid : tid % THREADS, sub = R == 1 ? 0 : tid / THREADS;
   const int chunks = a.C / VEC;
   float w[N][VEC], dw[N][VEC], db[N][VEC];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int c = t + 64 * W * i;
+    const int c = t + THREADS * i;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) { w[i][j] = 1.f; dw[i][j] = db[i][j] = 0.f; }
     if (a.w && c < chunks) load_w<T, VEC>(a.w, a.w32, c * VEC, w[i]);
@@ -162,7 +171,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_backward_kernel(con
     const T* dy = static_cast<const T*>(a.dy) + row * a.dy_row;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = t + 64 * W * i;
+      const int c = t + THREADS * i;
       if (c < chunks) {
         xr[i] = *reinterpret_cast<const raw*>(x + c * VEC);
         gr[i] = *reinterpret_cast<const raw*>(dy + c * VEC);
@@ -178,7 +187,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_backward_kernel(con
     const float r = rstd;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (t + 64 * W * i < chunks) {
+      if (t + THREADS * i < chunks) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           float xv, gv;
@@ -194,13 +203,13 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_backward_kernel(con
     }
     if (row + step < a.rows) fetch(row + step);
     if (a.dx) {
-      row_sum<W>(s1, s2, box, wave);
+      row_sum<W, L>(s1, s2, box, wave);
       s1 *= inv;
       s2 *= inv;
       T* dx = static_cast<T*>(a.dx) + row * a.dx_row;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int c = t + 64 * W * i;
+        const int c = t + THREADS * i;
         if (c < chunks) {
           float o[VEC];
 #pragma unroll
@@ -211,16 +220,16 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_backward_kernel(con
     }
   }
   if (!a.part) return;
-  if constexpr (R > 1) {                           // the block's waves one after the other, in their order
+  if constexpr (R > 1) {                           // the block's rows one after the other, in their order
     for (int k = 0; k < R; ++k) {
       if (sub == k) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            const int at = (i * VEC + j) * 64 + t;
+            const int at = (i * VEC + j) * L + t;
             share[at] = k ? share[at] + dw[i][j] : dw[i][j];
-            share[64 * N * VEC + at] = k ? share[64 * N * VEC + at] + db[i][j] : db[i][j];
+            share[L * N * VEC + at] = k ? share[L * N * VEC + at] + db[i][j] : db[i][j];
           }
       }
       __syncthreads();
@@ -230,14 +239,14 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void norm_backward_kernel(con
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        dw[i][j] = share[(i * VEC + j) * 64 + t];
-        db[i][j] = share[64 * N * VEC + (i * VEC + j) * 64 + t];
+        dw[i][j] = share[(i * VEC + j) * L + t];
+        db[i][j] = share[L * N * VEC + (i * VEC + j) * L + t];
       }
   }
   float* p = a.part + (size_t)blockIdx.x * 2 * a.C;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int c = t + 64 * W * i;
+    const int c = t + THREADS * i;
     if (c < chunks) {
       store<float, VEC < 4 ? VEC : 4>(p + c * VEC, dw[i]);
       store<float, VEC < 4 ? VEC : 4>(p + a.C + c * VEC, db[i]);
@@ -346,11 +355,17 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const NormArgs a) {
 }
 
 // ---- which instance takes a width: VEC entries per access, N accesses per thread, W waves per row; N = 0: the wide kernels
-struct Choice { int vec, n, w; };
+struct Choice { int vec, n, w, l; };
 Choice choose(int C, int size, bool aligned, int most) {         // most: entries of a row per thread
   Choice k;
   k.vec = aligned ? 16 / size : 1;
   const int64_t chunks = ((int64_t)C + k.vec - 1) / k.vec;
+  k.l = 64;
+  if (chunks <= 32) {                              // several rows to a wave (50000 x 192 bf16: forward 18 -> 12 us, backward 24 -> 19)
+    k.n = k.w = 1;
+    k.l = chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;
+    return k;
+  }
   for (int w : {1, 4, 16}) {
     k.w = w;
     for (int n = 1; n <= most / k.vec; n *= 2) {
@@ -366,7 +381,7 @@ Choice choose(int C, int size, bool aligned, int most) {         // most: entrie
 // little, and more blocks keep more loads on their way (50000 x 192: 24 us with 1024, 27 with 512).
 int backward_blocks(int64_t rows, int C, const Choice& k) {
   if (k.n == 0) return (int)max((int64_t)1, min((int64_t)64, rows));
-  const int per = k.w >= 4 ? 1 : 4 / k.w;
+  const int per = k.w >= 4 ? 1 : 256 / k.l;
   const int64_t most = k.w == 16 ? 256 : C <= 256 ? 1024 : 512;
   return (int)max((int64_t)1, min((rows + per - 1) / per, most));
 }
@@ -374,28 +389,33 @@ int backward_blocks(int64_t rows, int C, const Choice& k) {
 // on four waves with 32, 148 on sixteen with 16; 24571 x 4096 bf16: 92 on four waves, 96 on one with 64)
 constexpr int FORWARD = 32, BACKWARD = 16;
 
-template <class T, int VEC, int N, int W>
+template <class T, int VEC, int N, int W, int L>
 void launch_one(const NormArgs& a, bool backward, hipStream_t s) {
-  constexpr int R = W >= 4 ? 1 : 4 / W, threads = W > 4 ? 64 * W : 256;
+  constexpr int R = W >= 4 ? 1 : 256 / L, threads = W > 4 ? 64 * W : 256;
   if (backward) {
-    if constexpr (N * VEC <= BACKWARD) hipLaunchKernelGGL((norm_backward_kernel<T, VEC, N, W>), dim3(a.blocks), dim3(threads), 0, s, a);
-  } else hipLaunchKernelGGL((norm_forward_kernel<T, VEC, N, W>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(threads), 0, s, a);
+    if constexpr (N * VEC <= BACKWARD) hipLaunchKernelGGL((norm_backward_kernel<T, VEC, N, W, L>), dim3(a.blocks), dim3(threads), 0, s, a);
+  } else hipLaunchKernelGGL((norm_forward_kernel<T, VEC, N, W, L>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(threads), 0, s, a);
 }
 template <class T, int VEC, int N>
-void launch_w(const NormArgs& a, int w, bool backward, hipStream_t s) {
-  if (w == 1) launch_one<T, VEC, N, 1>(a, backward, s);
-  else if (w == 4) launch_one<T, VEC, N, 4>(a, backward, s);
-  else launch_one<T, VEC, N, 16>(a, backward, s);
+void launch_w(const NormArgs& a, const Choice& k, bool backward, hipStream_t s) {
+  if constexpr (N == 1) {
+    if (k.l == 8) return launch_one<T, VEC, 1, 1, 8>(a, backward, s);
+    if (k.l == 16) return launch_one<T, VEC, 1, 1, 16>(a, backward, s);
+    if (k.l == 32) return launch_one<T, VEC, 1, 1, 32>(a, backward, s);
+  }
+  if (k.w == 1) launch_one<T, VEC, N, 1, 64>(a, backward, s);
+  else if (k.w == 4) launch_one<T, VEC, N, 4, 64>(a, backward, s);
+  else launch_one<T, VEC, N, 16, 64>(a, backward, s);
 }
 template <class T, int VEC>
-void launch_n(const NormArgs& a, int n, int w, bool backward, hipStream_t s) {
+void launch_n(const NormArgs& a, const Choice& k, bool backward, hipStream_t s) {
   constexpr int most = (FORWARD > BACKWARD ? FORWARD : BACKWARD) / VEC;
-  if (n == 1) return launch_w<T, VEC, 1>(a, w, backward, s);
-  if constexpr (most >= 2) { if (n == 2) return launch_w<T, VEC, 2>(a, w, backward, s); }
-  if constexpr (most >= 4) { if (n == 4) return launch_w<T, VEC, 4>(a, w, backward, s); }
-  if constexpr (most >= 8) { if (n == 8) return launch_w<T, VEC, 8>(a, w, backward, s); }
-  if constexpr (most >= 16) { if (n == 16) return launch_w<T, VEC, 16>(a, w, backward, s); }
-  if constexpr (most >= 32) { if (n == 32) return launch_w<T, VEC, 32>(a, w, backward, s); }
+  if (k.n == 1) return launch_w<T, VEC, 1>(a, k, backward, s);
+  if constexpr (most >= 2) { if (k.n == 2) return launch_w<T, VEC, 2>(a, k, backward, s); }
+  if constexpr (most >= 4) { if (k.n == 4) return launch_w<T, VEC, 4>(a, k, backward, s); }
+  if constexpr (most >= 8) { if (k.n == 8) return launch_w<T, VEC, 8>(a, k, backward, s); }
+  if constexpr (most >= 16) { if (k.n == 16) return launch_w<T, VEC, 16>(a, k, backward, s); }
+  if constexpr (most >= 32) { if (k.n == 32) return launch_w<T, VEC, 32>(a, k, backward, s); }
 }
 template <class T>
 void launch(const NormArgs& a, const Choice& k, bool backward, hipStream_t s) {
@@ -405,8 +425,8 @@ void launch(const NormArgs& a, const Choice& k, bool backward, hipStream_t s) {
       if (a.dx) hipLaunchKernelGGL((norm_backward_wide_kernel<T>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);
       if (a.part) hipLaunchKernelGGL((norm_columns_kernel<T>), dim3((a.C + 255) / 256, a.blocks), dim3(256), 0, s, a);
     }
-  } else if (k.vec == 1) launch_n<T, 1>(a, k.n, k.w, backward, s);
-  else launch_n<T, 16 / (int)sizeof(T)>(a, k.n, k.w, backward, s);
+  } else if (k.vec == 1) launch_n<T, 1>(a, k, backward, s);
+  else launch_n<T, 16 / (int)sizeof(T)>(a, k, backward, s);
   if (backward && a.part) hipLaunchKernelGGL((norm_join_kernel<T>), dim3((2 * a.C + 31) / 32), dim3(1024), 0, s, a);
 }
 
