@@ -489,7 +489,7 @@ extern "C" int ac_layer_norm_backward(const ac_norm_args* p, void* ws, size_t ws
   a.rows = p->rows; a.C = p->width; a.w32 = p->weight_type == AC_F32;
   const size_t need = ac_layer_norm_backward_workspace_bytes(p);
   if (need && (!ws || ws_bytes < need)) return ac_fail(AC_EWORKSPACE, "ac_layer_norm_backward: workspace %zu < %zu", ws ? ws_bytes : (size_t)0, need);
-  AC_REQUIRE(((uintptr_t)ws & 3) == 0, "ac_layer_norm_backward: misaligned workspace");
+  AC_REQUIRE(!need || ((uintptr_t)ws & 15) == 0, "ac_layer_norm_backward: the workspace must be 16-byte aligned");
   if (!p->dx && !p->dweight && !p->dbias) return AC_OK;
   const bool al = aligned16(p, {p->x, p->dy, p->dx}, {p->x_row, p->dy_row, p->dx_row});
   const Choice k = choose(p->width, size, al, BACKWARD);

@@ -1113,7 +1113,8 @@ def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, c
         out = _fresh(q)
         os = (heads * dim, dim)
     else:
-        _, os = _heads(out, "out", like)
+        _heads(out, "out", like)
+        os = _strides(out)
         if out.shape != shape:
             raise ValueError("out must be %s, got %s" % (tuple(shape), tuple(out.shape)))
         _writable(out, "out")
@@ -1134,7 +1135,6 @@ def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, c
     if (qp | kp | vp | (qs[0] | qs[1] | ks[0] | ks[1] | vs[0] | vs[1]) * size) & 15:
         q, k, v = (t if _aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
         qp, kp, vp, qs, ks, vs = q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q), _strides(k), _strides(v)
-        os = _strides(out)
     if keys == 1:
         ks, vs = (0, ks[1]), (0, vs[1])
     args = _pack_attention(qp, kp, vp, out.data_ptr(), sums.data_ptr() if want_sums else 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],

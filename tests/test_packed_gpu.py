@@ -281,6 +281,19 @@ def test_attention_strides_and_alignment(dev, kind):
     _check_attention(acnative.attention_packed(db[:, :H], db[:, H:H + 1].expand(T, G, D), db[:, H + G:], ds), None, ref1, kind, D, "broadcast")
 
 
+def test_attention_single_token_with_odd_strides(dev):
+    """A tensor of one token or one head may carry any stride for that axis."""
+    base = _randn((3, 5, 64), 1, "bf16").to(dev)
+    q = base.as_strided((1, 5, 64), (321, 64, 1))
+    out = torch.zeros(400, dtype=torch.bfloat16, device=dev).as_strided((1, 5, 64), (333, 64, 1))
+    starts = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    acnative.attention_packed(q, q, q, starts, out=out)
+    assert torch.equal(out, q)                                      # one key: its value
+    one = base[:, :1].as_strided((3, 1, 64), (320, 7, 1))
+    got = acnative.attention_packed(one, one, one, torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=dev))
+    assert torch.equal(got, one)
+
+
 def test_attention_is_the_same_every_time(dev):
     sq, sk = _starts([1, 5, 260]), _starts([3000, 900, 1500])
     args = [t.to(dev) for t in (_randn((266, 8, 128), 1, "bf16"), _randn((5400, 2, 128), 2, "bf16"), _randn((5400, 2, 128), 3, "bf16"), sq, sk)]
