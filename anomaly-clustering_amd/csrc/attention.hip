@@ -861,7 +861,8 @@ Plan make_plan(const ac_attention_args* p) {
   if (r.kind == 0 && bytes > 128 && p->tokens_q * (int64_t)p->heads / 256 < 8 * ac_device_cus()) r.kind = 3;
   r.rows = r.kind == 2 ? 32 : r.kind != 0 ? 128 : 256;
   r.keys = r.kind == 2 && wide && bytes <= 256 ? 128 : 64;
-  r.tiles = (int)((rows + r.rows - 1) / r.rows);
+  // (a launch may not have 2^32 threads: many sequences under a loose bound get fewer blocks, which walk over the tiles)
+  r.tiles = (int)max((int64_t)1, min((rows + r.rows - 1) / r.rows, (1LL << 22) / pairs));
   // The key axis is split where the rows alone would leave CUs idle, into parts of 256 keys or more: so many that a CU gets about
   // four (16-bit; fp32 six) blocks.  Two waves on tiles of 64 keys, 64 KB of LDS: two blocks of a CU cover each other's start and
   // end.  16 queries on 64 .. 16000 keys, 32 / 8 heads of 128: 90 us, against 106 with four waves on 128 keys; 64 queries on 4096
@@ -879,8 +880,7 @@ int launch(const AttArgs& a, hipStream_t stream) {
   typedef Shape<T, NS, NQ, WQ, WK, KB> G;
   static unsigned long long done = 0;
   if (int rc = ac_set_max_lds(reinterpret_cast<const void*>(&packed_attention_kernel<T, NS, NQ, WQ, WK, KB>), G::LDS, &done)) return rc;
-  const int64_t blocks = (int64_t)a.pairs * a.replicas * a.tiles * a.splits;
-  if (blocks >= (1LL << 31)) return ac_fail(AC_EINVAL, "ac_attention_packed: too many blocks");
+  const int64_t blocks = (int64_t)a.pairs * a.replicas * a.tiles * a.splits;       // under 2^24 (make_plan, check)
   hipLaunchKernelGGL((packed_attention_kernel<T, NS, NQ, WQ, WK, KB>), dim3((unsigned)blocks), dim3(G::THREADS), G::LDS, stream, a);
   return AC_OK;
 }
@@ -945,7 +945,7 @@ int check(const ac_attention_args* p) {
   AC_REQUIRE(p->tokens_q * (int64_t)(p->heads / p->kv_heads) + 256 < (1LL << 31) && p->tokens_k + 256 < (1LL << 31) && p->tokens_q * (int64_t)p->heads < (1LL << 32),
              "ac_attention_packed: too many tokens");
   AC_REQUIRE(p->scale - p->scale == 0.f, "ac_attention_packed: the scale is not finite");
-  AC_REQUIRE((int64_t)p->sequences * p->kv_heads < (1LL << 27), "ac_attention_packed: too many sequences");
+  AC_REQUIRE((int64_t)p->sequences * p->kv_heads < (1LL << 21), "ac_attention_packed: too many sequences (2^21 with one key head)");
   return AC_OK;
 }
 

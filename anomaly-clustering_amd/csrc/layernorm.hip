@@ -417,17 +417,40 @@ void launch_n(const NormArgs& a, const Choice& k, bool backward, hipStream_t s) 
   if constexpr (most >= 16) { if (k.n == 16) return launch_w<T, VEC, 16>(a, k, backward, s); }
   if constexpr (most >= 32) { if (k.n == 32) return launch_w<T, VEC, 32>(a, k, backward, s); }
 }
+// One thread block or part of one per row (the forward pass, the wide kernels' dx); a launch may not have 2^32 threads: 2^28 in each,
+// one after the other
+template <class T, class F>
+void by_rows(const NormArgs& all, int threads, F launch_rows) {
+  const int64_t most = (1LL << 28) / threads;
+  for (int64_t r = 0; r < all.rows; r += most) {
+    NormArgs a = all;
+    a.rows = min(all.rows - r, most);
+    a.x = static_cast<const T*>(all.x) + r * all.x_row;
+    if (all.dy) a.dy = static_cast<const T*>(all.dy) + r * all.dy_row;
+    if (all.y) a.y = static_cast<T*>(all.y) + r * all.y_row;
+    if (all.dx) a.dx = static_cast<T*>(all.dx) + r * all.dx_row;
+    if (all.mean) { a.mean = all.mean + r; a.rstd = all.rstd + r; }
+    if (all.mean_in) { a.mean_in = all.mean_in + r; a.rstd_in = all.rstd_in + r; }
+    launch_rows(a);
+  }
+}
 template <class T>
-void launch(const NormArgs& a, const Choice& k, bool backward, hipStream_t s) {
+void launch(const NormArgs& all, const Choice& k, bool backward, hipStream_t s) {
   if (k.n == 0) {
-    if (!backward) hipLaunchKernelGGL((norm_forward_wide_kernel<T>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);
+    if (!backward) by_rows<T>(all, 1024, [&](const NormArgs& a) { hipLaunchKernelGGL((norm_forward_wide_kernel<T>), dim3((unsigned)a.rows), dim3(1024), 0, s, a); });
     else {
-      if (a.dx) hipLaunchKernelGGL((norm_backward_wide_kernel<T>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);
-      if (a.part) hipLaunchKernelGGL((norm_columns_kernel<T>), dim3((a.C + 255) / 256, a.blocks), dim3(256), 0, s, a);
+      if (all.dx) by_rows<T>(all, 1024, [&](const NormArgs& a) { hipLaunchKernelGGL((norm_backward_wide_kernel<T>), dim3((unsigned)a.rows), dim3(1024), 0, s, a); });
+      if (all.part) hipLaunchKernelGGL((norm_columns_kernel<T>), dim3((all.C + 255) / 256, all.blocks), dim3(256), 0, s, all);
     }
-  } else if (k.vec == 1) launch_n<T, 1>(a, k, backward, s);
-  else launch_n<T, 16 / (int)sizeof(T)>(a, k, backward, s);
-  if (backward && a.part) hipLaunchKernelGGL((norm_join_kernel<T>), dim3((2 * a.C + 31) / 32), dim3(1024), 0, s, a);
+  } else {
+    auto one = [&](const NormArgs& a) {
+      if (k.vec == 1) launch_n<T, 1>(a, k, backward, s);
+      else launch_n<T, 16 / (int)sizeof(T)>(a, k, backward, s);
+    };
+    if (backward) one(all);                        // its blocks walk over the rows
+    else by_rows<T>(all, k.l * k.w, one);
+  }
+  if (backward && all.part) hipLaunchKernelGGL((norm_join_kernel<T>), dim3((2 * all.C + 31) / 32), dim3(1024), 0, s, all);
 }
 
 int check(const ac_norm_args* p, const char* what) {

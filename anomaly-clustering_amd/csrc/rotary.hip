@@ -189,11 +189,20 @@ extern "C" int ac_rotary(const ac_rotary_args* r, void* stream) {
   int64_t group = max((int64_t)1, min((int64_t)16, 1024 / per_token));
   while (group > 1 && (r->tokens + group - 1) / group < 4 * ac_device_cus()) group /= 2;
   a.group = (int)group;
-  const int64_t blocks = (r->tokens + group - 1) / group;
-  AC_REQUIRE(blocks < (1LL << 31), "ac_rotary: too many tokens");
   const size_t lds = (size_t)group * r->part * sizeof(float);                 // 16 x 1024 x 4 = 64 KB at most
-  if (r->type == AC_F32) launch_vec<float>(a, vec, half, (unsigned)blocks, lds, as_stream(stream));
-  else if (r->type == AC_F16) launch_vec<_Float16>(a, vec, half, (unsigned)blocks, lds, as_stream(stream));
-  else launch_vec<__bf16>(a, vec, half, (unsigned)blocks, lds, as_stream(stream));
+  // (a launch may not have 2^32 threads: 2^20 blocks of 256 each, one after the other)
+  const int64_t most = group << 20;
+  for (int64_t t = 0; t < r->tokens; t += most) {
+    a.tokens = min(r->tokens - t, most);
+    a.positions = static_cast<const uint8_t*>(r->positions) + t * (r->positions64 ? 8 : 4);
+    for (int i = 0; i < 2; ++i) if (a.heads[i]) {
+      a.src[i] = static_cast<const uint8_t*>(r->src[i]) + t * a.s_tok[i] * size;
+      a.dst[i] = static_cast<uint8_t*>(r->dst[i]) + t * a.d_tok[i] * size;
+    }
+    const unsigned blocks = (unsigned)((a.tokens + group - 1) / group);
+    if (r->type == AC_F32) launch_vec<float>(a, vec, half, blocks, lds, as_stream(stream));
+    else if (r->type == AC_F16) launch_vec<_Float16>(a, vec, half, blocks, lds, as_stream(stream));
+    else launch_vec<__bf16>(a, vec, half, blocks, lds, as_stream(stream));
+  }
   return ac_check_launch("ac_rotary");
 }

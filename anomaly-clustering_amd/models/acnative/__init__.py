@@ -1081,7 +1081,8 @@ def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, c
     q [tokens, heads, dim], k and v [key tokens, kv_heads, dim], heads a multiple of kv_heads; float32, float16 or bfloat16;
     dim a multiple of 8 up to 256.  Sequence s is the rows starts_q[s] .. starts_q[s + 1] of q and starts_k[s] .. of k and v
     (int32 [sequences + 1] on the device; sequence_starts makes them); starts_k=None: the same as starts_q.  max_q / max_k: upper
-    bounds of the lengths - they shape the launch and never which rows are computed; None takes the number of tokens.  causal:
+    bounds of the lengths - they shape the launch and never which rows are computed; None takes the number of tokens, which starts a
+    block for every tile that there could be (4096 sequences of 64 tokens, 12 heads of 64 bf16: 6.6 ms, with max_q=64 0.73).  causal:
     query i of n sees key j of m where j <= i + m - n.  A row that sees no key, or none with a score above -inf, is zero; rows outside every sequence are left as they
     were in `out` (without `out`: zero).  scale: 1 / sqrt(dim) unless given.  want_sums: also the fp32 [tokens, heads] logarithm of
     each row's sum of exponentials (-inf for a row that sees no key, and outside every sequence).

@@ -363,7 +363,7 @@ int ac_rotary(const ac_rotary_args* args, void* stream);
  * & 1 makes them zero in out, clear & 2 -inf in sums.
  * starts_q, starts_k: int32 [sequences + 1] on the device, not decreasing, clamped there to 0 .. tokens.  max_q, max_k: upper bounds of the
  * lengths, used for the launch's shape alone (too small a bound costs time, not rows).  sums (nullable): fp32 [tokens_q,
- * heads], the natural logarithm of each row's sum of exponentials.  out must not overlap q, k or v. */
+ * heads], the natural logarithm of each row's sum of exponentials.  out must not overlap q, k or v.  sequences * kv_heads < 2^21. */
 typedef struct ac_attention_args {
   const void *q, *k, *v; void* out; float* sums;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;

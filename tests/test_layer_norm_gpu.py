@@ -198,3 +198,27 @@ def test_same_bits_every_time_and_in_a_graph(dev):
         assert all(torch.equal(p, q) for p, q in zip(out, step()))
         x.mul_(1.5)
         torch.cuda.synchronize()
+
+
+def test_more_rows_than_one_launch_takes(dev):
+    n = (1 << 25) + 5                                               # 8 threads to a row, 2^28 to a launch
+    gen = torch.Generator(device=dev).manual_seed(5)
+    x = torch.randn((n, 3), generator=gen, device=dev).bfloat16()
+    w = torch.randn(3, generator=gen, device=dev)
+    y, mean, rstd = acnative.layer_norm(x, w, w, want_stats=True)
+    for a, b in ((0, 9), ((1 << 25) - 7, n)):
+        part = acnative.layer_norm(x[a:b], w, w, want_stats=True)
+        for whole, p in zip((y, mean, rstd), part):
+            assert torch.equal(whole[a:b], p)
+
+
+def test_more_wide_rows_than_one_launch_takes(dev):
+    n, C = (1 << 18) + 3, 16392                                     # 1024 threads to a row; one row taken n times
+    gen = torch.Generator(device=dev).manual_seed(6)
+    x, dy = (torch.randn((1, C), generator=gen, device=dev).bfloat16() for _ in range(2))
+    w = torch.randn(C, generator=gen, device=dev)
+    _, mean, rstd = acnative.layer_norm(x, w, w, want_stats=True)
+    one = acnative.layer_norm_backward(dy, x, w, mean, rstd, want=(True, False, False))[0]
+    dx = acnative.layer_norm_backward(dy.expand(n, C), x.expand(n, C), w, mean.repeat(n), rstd.repeat(n), want=(True, False, False))[0]
+    for i in (0, (1 << 18) - 1, 1 << 18, n - 1):
+        assert torch.equal(dx[i], one[0]), i

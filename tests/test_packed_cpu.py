@@ -154,3 +154,10 @@ def test_layer_norm_backward_refuses_and_asks_for_its_workspace():
         acnative.layer_norm(torch.zeros(4, 8))
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         acnative.layer_norm_backward(torch.zeros(4, 8), torch.zeros(4, 8), None, torch.zeros(4), torch.zeros(4))
+
+
+def test_attention_refuses_more_pairs_than_a_launch_takes():
+    lib = acnative.lib()
+    assert lib.ac_attention_packed(ctypes.byref(_attention(sequences=1 << 20)), None, 0, None) == 1      # two key heads
+    assert "too many sequences" in lib.ac_last_error().decode()
+    assert lib.ac_attention_packed_workspace_bytes(ctypes.byref(_attention(sequences=1 << 20))) == 0

@@ -516,3 +516,33 @@ def test_wrappers_refuse_what_they_say(dev):
         with pytest.raises(error):
             call()
     assert acnative.attention_packed(x, x, x, starts, max_q=10 ** 12, max_k=10 ** 12).shape == x.shape
+
+
+def test_rotary_more_tokens_than_one_launch_takes(dev):
+    n = (16 << 20) + 37                                             # 16 tokens to a block, 2^20 blocks to a launch
+    gen = torch.Generator(device=dev).manual_seed(5)
+    q = torch.randn((n, 1, 2), generator=gen, device=dev).bfloat16()
+    p = torch.randint(0, 4000, (n,), generator=gen, device=dev, dtype=torch.int32)
+    f = torch.tensor([0.37], dtype=torch.float64, device=dev)
+    got = acnative.rotary(q, None, p, f)
+    got = got[0] if isinstance(got, tuple) else got
+    for a, b in ((0, 100), ((16 << 20) - 60, n)):
+        part = acnative.rotary(q[a:b], None, p[a:b].contiguous(), f)
+        assert torch.equal(got[a:b], part[0] if isinstance(part, tuple) else part)
+
+
+def test_attention_many_sequences_without_bounds(dev):
+    """The bound of every sequence is then the number of tokens: more blocks than a launch has, so they walk over the tiles."""
+    lengths = [50000] + [(37 * i) % 131 for i in range(2000)]
+    starts = _starts(lengths).to(dev)
+    T = sum(lengths)
+    gen = torch.Generator(device=dev).manual_seed(3)
+    qkv = torch.randn((T, 36, 64), generator=gen, device=dev).bfloat16()
+    q, k, v = qkv[:, :12], qkv[:, 12:24], qkv[:, 24:]
+    got = acnative.attention_packed(q, k, v, starts)
+    # the same tiles and keys in the same order: the same bits
+    n = 50000
+    one = acnative.attention_packed(q[:n], k[:n], v[:n], torch.tensor([0, n], dtype=torch.int32, device=dev))
+    assert torch.equal(got[:n], one)
+    rest = acnative.attention_packed(q[n:], k[n:], v[n:], starts[1:] - n, max_q=130, max_k=130)
+    assert torch.equal(got[n:], rest)
