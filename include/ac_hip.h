@@ -50,7 +50,7 @@ extern "C" {
 /* ABI revision: changes whenever an entry point changes meaning or a new one is added; a binding checks it at load
  * time (models/acnative does: a stale library under a newer binding - or the reverse - fails there, not in a kernel).
  * 500 = round 5: ac_alpha_softmax is the 7-argument form again, the fp32 copy moved to ac_alpha_softmax_f32.
- * 600 = round 6: ac_patch_aggregate_hl32 / ac_patch_aggregate_hl32_supported added.  The entry points for packed sequences
+ * 600: ac_patch_aggregate_hl32 / ac_patch_aggregate_hl32_supported added.  The entry points for packed sequences
  * came later and left it: nothing else changed, and a binding that misses one fails on its name. */
 #define AC_ABI_VERSION 600
 int ac_version(void);
