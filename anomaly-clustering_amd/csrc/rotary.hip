@@ -8,7 +8,7 @@
 // every head; products and sums are fp32, the result is rounded to the tensor's type once.
 //
 // Bound: memory; each element is read once and written once, nothing else is of size.  65536 tokens x 40 heads of 128 in bf16
-// (1.34 GB): 238 us, 5.6 TB/s, where a copy of 1 GB reaches 5.2.
+// (1.34 GB), half of each turning: 238 us, 5.6 TB/s, where a copy of 1 GB reaches 5.2.
 #include "common.h"
 
 namespace {
@@ -58,6 +58,30 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   const int n = (int)min((int64_t)a.group, a.tokens - t0);
   float* const cosines = table;
   float* const sines = table + a.group * pairs;
+  const int turning = HALF ? pairs / VEC : a.part / VEC, units = turning + (a.dim - a.part) / VEC;
+  const int wide = min(units, 256), rows_at_once = 256 / wide;
+  const int r0 = threadIdx.x / wide, u0 = threadIdx.x - r0 * wide;
+  typedef typename Pack<T, VEC>::type raw;
+  const int heads = a.heads[0] + a.heads[1], rows = n * heads;
+  const int before = a.offset / VEC;
+  // units in the order of their places (neighbouring lanes, neighbouring addresses); the half layout's skip the second entries
+  auto turns = [&](int u) { return u >= before && u - before < turning; };
+  raw x, y;
+  T* dst;
+  int tok;
+  auto fetch = [&](int u, int row) {
+    const int at = HALF && u - before >= turning ? u * VEC + pairs : u * VEC;
+    tok = row / heads;
+    const int hh = row - tok * heads, which = hh >= a.heads[0], h = which ? hh - a.heads[0] : hh;
+    const T* src = static_cast<const T*>(a.src[which]) + (t0 + tok) * a.s_tok[which] + h * a.s_head[which] + at;
+    dst = static_cast<T*>(a.dst[which]) + (t0 + tok) * a.d_tok[which] + h * a.d_head[which] + at;
+    x = *reinterpret_cast<const raw*>(src);
+    if (HALF && turns(u)) y = *reinterpret_cast<const raw*>(src + pairs);
+  };
+  // The first entries are on their way while the table is made: 65536 tokens x 40 heads of 128 bf16, half of each interleaved, 285 ->
+  // 238 us; 25120 x 24 heads of 64 fp32 55 -> 49; all of each, half layout, 236 (two rows at a time, behind the table) -> 242.
+  const bool mine = r0 < rows_at_once && u0 < units && r0 < rows;
+  if (mine) fetch(u0, r0);
   for (int i = threadIdx.x; i < n * pairs; i += 256) {
     const int t = i / pairs, p = i - t * pairs;
     const int64_t at = (int64_t)(p / per_axis) * a.pos_axis + t0 + t;
@@ -68,67 +92,37 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     sines[i] = (a.inverse ? -s : s) * a.amplitude;
   }
   __syncthreads();
-  const int turning = HALF ? pairs / VEC : a.part / VEC, units = turning + (a.dim - a.part) / VEC;
-  const int wide = min(units, 256), rows_at_once = 256 / wide;
-  const int r0 = threadIdx.x / wide, u0 = threadIdx.x - r0 * wide;
-  if (r0 >= rows_at_once) return;
-  typedef typename Pack<T, VEC>::type raw;
-  const int heads = a.heads[0] + a.heads[1], rows = n * heads;
+  if (!mine) return;
   for (int u = u0; u < units; u += wide) {
-    // units in the order of their places (neighbouring lanes, neighbouring addresses); the half layout's skip the second entries
-    const int before = a.offset / VEC, turn = u - before;
-    const bool turns = turn >= 0 && turn < turning;
-    const int at = HALF && turn >= turning ? u * VEC + pairs : u * VEC;
-    // two rows at a time where a unit is two accesses, their loads first (65536 x 40 heads of 128: 238 us with two, 255 with four, 387
-    // with eight, which cost waves; interleaved, half of each head: 286 us with one, 308 with two)
-    constexpr int U = HALF ? 2 : 1;
-    for (int row = r0; row < rows; row += U * rows_at_once) {
-      raw x[U], y[U];
-      T* dst[U];
-      int tok[U];
+    for (int row = r0; row < rows; row += rows_at_once) {
+      if (u != u0 || row != r0) fetch(u, row);
+      raw* const out = reinterpret_cast<raw*>(dst);
+      if (!turns(u)) { *out = x; continue; }
+      constexpr int P = HALF ? VEC : VEC / 2;      // pairs of a unit
+      const float* c = cosines + tok * pairs + (u - before) * P;
+      const float* s = sines + tok * pairs + (u - before) * P;
+      if constexpr (HALF) {
+        raw ox, oy;
+        if constexpr (VEC == 1) {
+          ox = (T)((float)x * c[0] - (float)y * s[0]);
+          oy = (T)((float)y * c[0] + (float)x * s[0]);
+        } else {
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int rj = row + j * rows_at_once;
-        const int t = rj / heads, hh = rj - t * heads, which = hh >= a.heads[0], h = which ? hh - a.heads[0] : hh;
-        tok[j] = rj < rows ? t : -1;
-        if (rj < rows) {
-          const T* src = static_cast<const T*>(a.src[which]) + (t0 + t) * a.s_tok[which] + h * a.s_head[which] + at;
-          dst[j] = static_cast<T*>(a.dst[which]) + (t0 + t) * a.d_tok[which] + h * a.d_head[which] + at;
-          x[j] = *reinterpret_cast<const raw*>(src);
-          if (HALF && turns) y[j] = *reinterpret_cast<const raw*>(src + pairs);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        if (tok[j] < 0) continue;
-        raw* const out = reinterpret_cast<raw*>(dst[j]);
-        if (!turns) { *out = x[j]; continue; }
-        constexpr int P = HALF ? VEC : VEC / 2;    // pairs of a unit
-        const float* c = cosines + tok[j] * pairs + turn * P;
-        const float* s = sines + tok[j] * pairs + turn * P;
-        if constexpr (HALF) {
-          raw ox, oy;
-          if constexpr (VEC == 1) {
-            ox = (T)((float)x[j] * c[0] - (float)y[j] * s[0]);
-            oy = (T)((float)y[j] * c[0] + (float)x[j] * s[0]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              ox[i] = (T)((float)x[j][i] * c[i] - (float)y[j][i] * s[i]);
-              oy[i] = (T)((float)y[j][i] * c[i] + (float)x[j][i] * s[i]);
-            }
+          for (int i = 0; i < VEC; ++i) {
+            ox[i] = (T)((float)x[i] * c[i] - (float)y[i] * s[i]);
+            oy[i] = (T)((float)y[i] * c[i] + (float)x[i] * s[i]);
           }
-          *out = ox;
-          *reinterpret_cast<raw*>(dst[j] + pairs) = oy;
-        } else if constexpr (VEC >= 2) {
-          raw o;
-#pragma unroll
-          for (int i = 0; i < P; ++i) {
-            o[2 * i] = (T)((float)x[j][2 * i] * c[i] - (float)x[j][2 * i + 1] * s[i]);
-            o[2 * i + 1] = (T)((float)x[j][2 * i + 1] * c[i] + (float)x[j][2 * i] * s[i]);
-          }
-          *out = o;
         }
+        *out = ox;
+        *reinterpret_cast<raw*>(dst + pairs) = oy;
+      } else if constexpr (VEC >= 2) {
+        raw o;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          o[2 * i] = (T)((float)x[2 * i] * c[i] - (float)x[2 * i + 1] * s[i]);
+          o[2 * i + 1] = (T)((float)x[2 * i + 1] * c[i] + (float)x[2 * i] * s[i]);
+        }
+        *out = o;
       }
     }
   }
@@ -183,7 +177,7 @@ extern "C" int ac_rotary(const ac_rotary_args* r, void* stream) {
   a.positions = r->positions; a.pos_axis = r->position_axis; a.pos64 = r->positions64; a.freq = r->frequencies;
   a.tokens = r->tokens; a.dim = r->dim; a.part = r->part; a.offset = r->offset; a.axes = r->axes;
   a.amplitude = r->amplitude; a.inverse = r->inverse;
-  // tokens per block: about 1024 accesses for its 256 threads (65536 tokens x 40 heads of 128, bf16, four rows at a time: 254 us with
+  // tokens per block: about 1024 accesses for its 256 threads (65536 tokens x 40 heads of 128, bf16, four rows at a time behind the table: 254 us with
   // 1024 or 2048, 267 with 4096, 284 with 8192), fewer where that would leave CUs idle
   const int64_t per_token = (int64_t)(r->heads[0] + r->heads[1]) * (r->dim / vec);
   int64_t group = max((int64_t)1, min((int64_t)16, 1024 / per_token));
