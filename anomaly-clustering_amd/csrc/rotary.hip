@@ -177,8 +177,8 @@ extern "C" int ac_rotary(const ac_rotary_args* r, void* stream) {
   a.positions = r->positions; a.pos_axis = r->position_axis; a.pos64 = r->positions64; a.freq = r->frequencies;
   a.tokens = r->tokens; a.dim = r->dim; a.part = r->part; a.offset = r->offset; a.axes = r->axes;
   a.amplitude = r->amplitude; a.inverse = r->inverse;
-  // tokens per block: about 1024 accesses for its 256 threads (65536 tokens x 40 heads of 128, bf16, four rows at a time behind the table: 254 us with
-  // 1024 or 2048, 267 with 4096, 284 with 8192), fewer where that would leave CUs idle
+  // tokens per block: about 1024 accesses for its 256 threads (65536 tokens x 40 heads of 128 bf16: 239 us with 512 or 1024, 254 with
+  // 2048; 25120 x 24 heads of 64 fp32: 52, 49, 50), fewer where that would leave CUs idle
   const int64_t per_token = (int64_t)(r->heads[0] + r->heads[1]) * (r->dim / vec);
   int64_t group = max((int64_t)1, min((int64_t)16, 1024 / per_token));
   while (group > 1 && (r->tokens + group - 1) / group < 4 * ac_device_cus()) group /= 2;
