@@ -1,10 +1,8 @@
-"""What is measured of the operators for packed sequences: layer norm, rotary positions and attention.
+"""What is measured of the operators for packed sequences: rotary positions and attention.
 
-A backbone that reads images of their own sizes (or prompts of their own lengths) has its sequences packed: one row per
-token, sequence s in the rows starts[s] .. starts[s + 1].  Three operators work on them, the attention half of a block:
+A backbone that reads images of their own sizes (or prompts of their own lengths) has its sequences packed: one
+[tokens, heads, dim] tensor, sequence s in the rows starts[s] .. starts[s + 1].  Two operators work on it:
 
-norm       y = (x - mean) / sqrt(variance + eps) w + b for each row; with its backward pass (dx, and dw and db summed over
-           the rows), for a backbone whose norms are tuned to the images at hand.
 rotary     pair i of a head turns by angle = position * frequency[i]:  (a, b) -> m (a cos - b sin, a sin + b cos).  Pairs are
            (i, i + part / 2) in the half layout and (2 i, 2 i + 1) in the interleaved one; `part` entries of the head from
            `offset` on are turned, the others pass.  With two axes the first half of the pairs goes by the row of a patch in
@@ -18,7 +16,6 @@ import torch
 
 own = False
 
-EPS = 1e-6
 TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
 
 
@@ -33,32 +30,28 @@ def _attention(name, kind, heads, kv_heads, dim, queries, keys="", causal=False,
             "causal": causal, "sums": sums}
 
 
-def _norm(name, kind, weights, rows, width, backward):
-    return {"name": name, "op": "norm", "type": kind, "weights": weights, "rows": rows, "width": width, "backward": backward}
-
-
 def listed():
     return [
-        # one decoding step of 8 sequences
-        _norm("norm-step", "bf16", "bf16", 8, 4096, False),
-        # 32 images at the 224 grid, width 768, in the framework's own type, forward and backward
-        _norm("norm-images-fp32", "fp32", "fp32", 32 * 785, 768, True),
-        # a packed batch of prompts with an odd number of tokens, weights kept in 32 bits, forward and backward
-        _norm("norm-prompts", "bf16", "fp32", 24571, 4096, True),
         # one decoding step of 8 sequences, far into a stretched context: what counts is the latency of a launch
         _rotary("rotary-step", "bf16", 8, 16, 4, 128, 128, factor=8.0, far=30000),
         # eight 224 x 224 images at patch 8, twelve heads of 64, the framework's own type; rows and columns as two axes
         _rotary("rotary-images-fp32", "fp32", 8 * 785, 12, 12, 64, 64, axes=2, base=100.0, far=28),
-        # a long document read at once: positions where 32-bit angles have no digits left; neighbouring pairs, half of each head
-        _rotary("rotary-long", "bf16", 65536, 32, 8, 128, 64, layout="interleaved", offset=32, factor=16.0, original=8192, far=4000000),
+        # a packed batch of prompts, half of each head turned, neighbouring pairs
+        _rotary("rotary-prompts", "fp16", 24571, 32, 8, 128, 64, layout="interleaved", offset=32, far=8192),
+        # a long document read at once: positions where 32-bit angles have no digits left
+        _rotary("rotary-long", "bf16", 131072, 32, 8, 128, 128, factor=16.0, original=8192, far=4000000),
         # one small crop: 17 tokens
         _attention("attention-crop", "bf16", 12, 12, 64, "17"),
         # 32 images at the 224 grid as the ViT-B/8 backbone has them, in the framework's own type
         _attention("attention-images-fp32", "fp32", 12, 12, 64, "32*785"),
         # the same backbone in bf16 on images of their own sizes, 32 x 48 .. 384 x 384 pixels at patch 8 or 16
         _attention("attention-images", "bf16", 12, 12, 64, "8*785,1025,197,2305,25,577,1,1601,1297,442,2305,901"),
+        # a wider backbone with heads of 80, a few large images
+        _attention("attention-wide-heads", "fp16", 16, 16, 80, "3*4097,2305,3137"),
         # a batch of prompts, causal, four query heads to a key head
         _attention("attention-prompts", "bf16", 32, 8, 128, "4096,2777,1531,811,333,4001,64,1", causal=True, sums=True),
+        # prompts read on behind what their sequences hold already; one of them has nothing to add
+        _attention("attention-continued", "fp16", 16, 2, 128, "512,0,300,128,77", "6000,900,3300,128,8077", causal=True),
         # one long prompt
         _attention("attention-long", "bf16", 16, 4, 128, "16384", causal=True),
         # a decoding step: one query to each sequence
@@ -72,18 +65,13 @@ def _log(rng, low, high):
 
 
 def draw(rng):
-    kind, which = rng.choice(["bf16", "bf16", "fp16", "fp32"]), rng.random()
-    if which < 0.3:
-        width = rng.choice([64, 192, 384, 768, 1000, 1024, 1280, 4096, 5120, 8192]) if rng.random() < 0.7 else _log(rng, 16, 16384)
-        rows = 24571 * 4096 * 2 // (width * (4 if kind == "fp32" else 2)) - 1
-        case = _norm("", kind, rng.choice([kind, "fp32"]), _log(rng, 1, min(100000, rows)), width, rng.random() < 0.7)
-        return {k: v for k, v in case.items() if k != "name"}
-    if which < 0.55:
+    kind = rng.choice(["bf16", "bf16", "fp16", "fp32"])
+    if rng.random() < 0.4:
         dim = rng.choice([32, 64, 80, 96, 128, 128, 192, 256])
         kv_heads, axes = rng.choice([1, 2, 4, 8, 12]), rng.choice([1, 1, 2])
         part = dim if rng.random() < 0.5 else max(8, dim * rng.randint(1, 3) // 4 // 8 * 8)
-        rows = 65536 * 40 * 128 * 2 // (kv_heads * 5 * dim * (4 if kind == "fp32" else 2))
-        return {k: v for k, v in _rotary("", kind, _log(rng, 1, min(65536, rows)), kv_heads * rng.choice([1, 2, 4]), kv_heads, dim, part, axes=axes,
+        rows = 131072 * 40 * 128 * 2 // (kv_heads * 5 * dim * (4 if kind == "fp32" else 2))
+        return {k: v for k, v in _rotary("", kind, _log(rng, 1, min(131072, rows)), kv_heads * rng.choice([1, 2, 4]), kv_heads, dim, part, axes=axes,
                                          offset=rng.choice([0, (dim - part) // 8 * 8]), layout=rng.choice(["half", "interleaved"]),
                                          base=rng.choice([100.0, 10000.0, 500000.0]), factor=rng.choice([1.0, 4.0, 16.0]),
                                          far=_log(rng, 64, 4000000) if axes == 1 else _log(rng, 8, 256)).items() if k != "name"}
@@ -138,15 +126,8 @@ def _amplitude(case):
 
 def prepare(case, seed):
     g = torch.Generator("cuda").manual_seed(seed)
-    kind, state = TYPES[case["type"]], {"case": case}
-    if case["op"] == "norm":
-        R, C, weights = case["rows"], case["width"], TYPES[case["weights"]]
-        x = torch.randn(R, C, generator=g, device="cuda") * 1.3 + torch.randn(C, generator=g, device="cuda")  # channels with means of their own
-        state["x"], state["dy"] = x.to(kind), (torch.randn(R, C, generator=g, device="cuda") * 0.01).to(kind)
-        state["w"] = (1.0 + 0.2 * torch.randn(C, generator=g, device="cuda")).to(weights)
-        state["b"] = (0.1 * torch.randn(C, generator=g, device="cuda")).to(weights)
-        return state
-    H, G, D = case["heads"], case["kv_heads"], case["dim"]
+    kind, H, G, D = TYPES[case["type"]], case["heads"], case["kv_heads"], case["dim"]
+    state = {"case": case}
     if case["op"] == "rotary":
         T = case["tokens"]
         qkv = torch.randn(T, H + 2 * G, D, generator=g, device="cuda").to(kind)  # as one projection writes them
@@ -173,20 +154,6 @@ def prepare(case, seed):
     state["starts_k"] = torch.tensor([0] + keys).cumsum(0).to(device="cuda", dtype=torch.int32)
     state["max_q"], state["max_k"] = max(queries), max(keys)
     return state
-
-
-def _plain_norm(state):
-    x, w = state["x"].float(), state["w"].float()
-    off = x - x.mean(1, keepdim=True)
-    rstd = (off.square().mean(1, keepdim=True) + EPS).rsqrt()
-    unit = off * rstd
-    y = (unit * w + state["b"].float()).to(state["x"].dtype)
-    if not state["case"]["backward"]:
-        return y
-    dy = state["dy"].float()
-    g = dy * w
-    dx = rstd * (g - g.mean(1, keepdim=True) - unit * (g * unit).mean(1, keepdim=True))
-    return y, dx.to(state["x"].dtype), (dy * unit).sum(0).to(state["w"].dtype), dy.sum(0).to(state["w"].dtype)
 
 
 def _turn(x, cos, sin, case):
@@ -257,26 +224,16 @@ def run(state):
         if "anomaly-clustering_amd/models" not in sys.path:
             sys.path.insert(0, "anomaly-clustering_amd/models")  # the packages' folder, as PYTHONPATH has it
         import acnative
-        if case["op"] == "norm" and not case["backward"]:
-            return acnative.layer_norm(state["x"], state["w"], state["b"], eps=EPS)
-        if case["op"] == "norm":
-            y, mean, rstd = acnative.layer_norm(state["x"], state["w"], state["b"], eps=EPS, want_stats=True)
-            return (y,) + acnative.layer_norm_backward(state["dy"], state["x"], state["w"], mean, rstd)
         if case["op"] == "rotary":
             return acnative.rotary(state["q"], state["k"], state["positions"], state["frequencies"], layout=case["layout"], offset=case["offset"],
                                    amplitude=_amplitude(case))
         return acnative.attention_packed(state["q"], state["k"], state["v"], state["starts_q"], state["starts_k"], max_q=state["max_q"],
                                          max_k=state["max_k"], causal=case["causal"], want_sums=case["sums"])
-    return {"norm": _plain_norm, "rotary": _plain_rotary, "attention": _plain_attention}[case["op"]](state)
+    return _plain_rotary(state) if case["op"] == "rotary" else _plain_attention(state)
 
 
 def work(case):
     size = 4 if case["type"] == "fp32" else 2
-    if case["op"] == "norm":
-        n, vector = case["rows"] * case["width"], case["width"] * (4 if case["weights"] == "fp32" else 2)
-        # forward: x in, y out; backward: x and dy in, dx out, the statistics in between
-        return {"bytes": (2 + 3 * case["backward"]) * n * size + (2 + 3 * case["backward"]) * vector + 16 * case["rows"] * case["backward"],
-                "flops": (8 + 14 * case["backward"]) * n}
     H, G, D = case["heads"], case["kv_heads"], case["dim"]
     if case["op"] == "rotary":
         T = case["tokens"]
@@ -296,12 +253,6 @@ def work(case):
 
 def exact(case, seed):
     state = prepare(case, seed)
-    if case["op"] == "norm":
-        # the gradients by differentiating the definition
-        x, w, b = (state[k].double().requires_grad_() for k in ("x", "w", "b"))
-        variance, mean = torch.var_mean(x, dim=1, unbiased=False, keepdim=True)
-        y = (x - mean) / (variance + EPS).sqrt() * w + b
-        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), state["dy"].double()) if case["backward"] else y.detach()
     if case["op"] == "rotary":
         # in complex numbers: each pair times m e^(i angle)
         angle = torch.einsum("at,ap->tap", state["positions"].double(), state["frequencies"]).reshape(case["tokens"], 1, -1)
