@@ -150,8 +150,10 @@ extern "C" int ac_rotary(const ac_rotary_args* r, void* stream) {
   AC_REQUIRE(r->layout == AC_ROTARY_HALF || r->layout == AC_ROTARY_INTERLEAVED, "ac_rotary: unknown layout %d", r->layout);
   AC_REQUIRE(r->tokens >= 0 && r->heads[0] >= 1 && r->heads[1] >= 0, "ac_rotary: bad counts");
   AC_REQUIRE(r->dim >= 1 && r->dim <= 1024, "ac_rotary: head dim %d must be in 1 .. 1024", r->dim);
-  AC_REQUIRE(r->axes >= 1 && r->part >= 2 && r->part % (2 * r->axes) == 0, "ac_rotary: part=%d must be a positive multiple of 2 * axes (%d)", r->part, 2 * r->axes);
-  AC_REQUIRE(r->offset >= 0 && r->offset + r->part <= r->dim, "ac_rotary: entries %d .. %d lie outside a head of %d", r->offset, r->offset + r->part, r->dim);
+  AC_REQUIRE(r->axes >= 1 && r->part >= 2 && r->axes <= r->part / 2 && r->part % (2 * r->axes) == 0,
+             "ac_rotary: part=%d must be a positive multiple of 2 * axes (2 * %d)", r->part, r->axes);
+  AC_REQUIRE(r->offset >= 0 && r->part <= r->dim && r->offset <= r->dim - r->part, "ac_rotary: entries %d .. %lld lie outside a head of %d", r->offset,
+             (long long)r->offset + r->part, r->dim);
   AC_REQUIRE((int64_t)r->heads[0] + r->heads[1] <= 1 << 20, "ac_rotary: too many heads");
   if (r->tokens == 0) return AC_OK;
   AC_REQUIRE(r->positions && r->frequencies, "ac_rotary: null pointer");

@@ -161,3 +161,13 @@ def test_attention_refuses_more_pairs_than_a_launch_takes():
     assert lib.ac_attention_packed(ctypes.byref(_attention(sequences=1 << 20)), None, 0, None) == 1      # two key heads
     assert "too many sequences" in lib.ac_last_error().decode()
     assert lib.ac_attention_packed_workspace_bytes(ctypes.byref(_attention(sequences=1 << 20))) == 0
+
+
+@pytest.mark.parametrize("over,text", [({"offset": (1 << 31) - 2, "part": 2}, "outside a head"), ({"offset": (1 << 31) - 64}, "outside a head"),
+                                       ({"part": (1 << 31) - 2, "offset": 2}, "outside a head"), ({"axes": (1 << 31) - 1}, "multiple of 2"),
+                                       ({"axes": 1 << 30}, "multiple of 2"), ({"axes": (1 << 30) + 16}, "multiple of 2"), ({"axes": -1}, "multiple of 2")])
+def test_rotary_refuses_what_only_32_bits_would_let_through(over, text):
+    """offset + part and 2 * axes, formed in 32 bits, wrap around to values that pass."""
+    lib = acnative.lib()
+    assert lib.ac_rotary(ctypes.byref(_rotary(**over)), None) == 1
+    assert text in lib.ac_last_error().decode()
