@@ -942,7 +942,8 @@ int check(const ac_attention_args* p) {
   AC_REQUIRE(p->heads >= 1 && p->kv_heads >= 1 && p->heads % p->kv_heads == 0, "ac_attention_packed: %d heads cannot share %d key heads", p->heads, p->kv_heads);
   AC_REQUIRE(p->dim >= 8 && p->dim <= 256 && p->dim % 8 == 0, "ac_attention_packed: head dim %d must be a multiple of 8, 8 .. 256", p->dim);
   AC_REQUIRE(p->sequences >= 0 && p->tokens_q >= 0 && p->tokens_k >= 0, "ac_attention_packed: negative count");
-  AC_REQUIRE(p->tokens_q * (int64_t)(p->heads / p->kv_heads) + 256 < (1LL << 31) && p->tokens_k + 256 < (1LL << 31) && p->tokens_q * (int64_t)p->heads < (1LL << 32),
+  const int64_t most = (1LL << 31) - 256;                        // (each count first: their products then fit 64 bits)
+  AC_REQUIRE(p->tokens_q < most && p->tokens_k < most && p->tokens_q * (p->heads / p->kv_heads) < most && p->tokens_q * p->heads < (1LL << 32),
              "ac_attention_packed: too many tokens");
   AC_REQUIRE(p->scale - p->scale == 0.f, "ac_attention_packed: the scale is not finite");
   AC_REQUIRE((int64_t)p->sequences * p->kv_heads < (1LL << 21), "ac_attention_packed: too many sequences (2^21 with one key head)");

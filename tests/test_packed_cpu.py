@@ -171,3 +171,12 @@ def test_rotary_refuses_what_only_32_bits_would_let_through(over, text):
     lib = acnative.lib()
     assert lib.ac_rotary(ctypes.byref(_rotary(**over)), None) == 1
     assert text in lib.ac_last_error().decode()
+
+
+@pytest.mark.parametrize("over", [{"tokens_q": 1 << 62, "heads": 4, "kv_heads": 1}, {"tokens_k": (1 << 63) - 1}, {"tokens_q": (1 << 63) - 1, "heads": 2, "kv_heads": 1}])
+def test_attention_refuses_what_only_64_bits_would_let_through(over):
+    """tokens_q * heads and tokens_k + a tile, formed in 64 bits, wrap around to values that pass."""
+    lib = acnative.lib()
+    assert lib.ac_attention_packed(ctypes.byref(_attention(**over)), None, 0, None) == 1
+    assert "too many tokens" in lib.ac_last_error().decode()
+    assert lib.ac_attention_packed_workspace_bytes(ctypes.byref(_attention(**over))) == 0
