@@ -42,7 +42,7 @@ def _deps_mtime():
 
 
 def build(force=False, verbose=True, experimental=False):
-    """Compile if the library is missing or older than any source/header.  Returns the path.
+    """Compile if the library is missing, older than any source/header or of other flags.  Returns the path.
     experimental=True builds libac_hip_experimental.so with -DAC_EXPERIMENTAL instead: the superseded GEMM
     generations under scratch/gemm_generations/ become selectable through ac_set_gemm_policy(101..109) for same-box
     A/B runs (load it with AC_LIB=...).  The product library never contains them."""
@@ -51,14 +51,26 @@ def build(force=False, verbose=True, experimental=False):
     return _build(force, verbose, LIB, OBJ_DIR, [])
 
 
+def _flags_record(extra):
+    """What a library was compiled with, the tree's own folders relative to this file (a copy of the tree has the same record)."""
+    flat = FLAGS + ["%s: %s" % (name, " ".join(flags)) for name, flags in sorted(FILE_FLAGS.items())] + extra
+    return "".join((os.path.relpath(f, HERE) if os.path.isabs(f) else f) + "\n" for f in flat)
+
+
 def _build(force, verbose, LIB, OBJ_DIR, extra):
     srcs = _sources()
-    if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= _deps_mtime():
-        return LIB
+    # flags carry correctness too (no packed fp32 instructions): a library without their record, or of others, is stale
+    record, wanted = os.path.join(OBJ_DIR, os.path.basename(LIB) + ".flags"), _flags_record(extra)
+    if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= _deps_mtime() and os.path.exists(record):
+        with open(record) as f:
+            if f.read() == wanted:
+                return LIB
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     if not os.path.exists(hipcc):
         raise RuntimeError("hipcc not found at %s: cannot build libac_hip.so" % hipcc)
     os.makedirs(OBJ_DIR, exist_ok=True)
+    if os.path.exists(record):
+        os.remove(record)
 
     def compile_one(src):
         obj = os.path.join(OBJ_DIR, os.path.basename(src)[:-4] + ".o")
@@ -76,6 +88,8 @@ def _build(force, verbose, LIB, OBJ_DIR, extra):
                        capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("link failed:\n%s\n%s" % (r.stdout, r.stderr))
+    with open(record, "w") as f:
+        f.write(wanted)
     if verbose:
         print("built", LIB)
     return LIB
