@@ -49,7 +49,8 @@ __device__ inline void cos_sin(double x, float& c, float& s) {
 template <class T, int VEC> struct Pack { typedef T type __attribute__((ext_vector_type(VEC))); };
 template <class T> struct Pack<T, 1> { typedef T type; };
 // One block: `group` tokens, all heads of q and k.  A unit is VEC elements of a head that pass, VEC neighbours that turn
-// (interleaved) or VEC pairs (half); thread -> (row, unit), a row being one head of one token.
+// (interleaved) or VEC pairs (half); thread -> (row, unit), a row being one head of one token.  With VEC = 1 an interleaved pair
+// is a unit of two accesses too (one thread has to own both entries: q may turn in place).
 template <class T, int VEC, bool HALF>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   extern __shared__ float table[];               // [group][pairs] cosines, then as many sines
@@ -58,25 +59,28 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   const int n = (int)min((int64_t)a.group, a.tokens - t0);
   float* const cosines = table;
   float* const sines = table + a.group * pairs;
-  const int turning = HALF ? pairs / VEC : a.part / VEC, units = turning + (a.dim - a.part) / VEC;
+  constexpr bool TWO = HALF || VEC == 1;         // a unit that turns has its second entries elsewhere
+  const int apart = HALF ? pairs : 1;
+  const int turning = TWO ? pairs / VEC : a.part / VEC, units = turning + (a.dim - a.part) / VEC;
   const int wide = min(units, 256), rows_at_once = 256 / wide;
   const int r0 = threadIdx.x / wide, u0 = threadIdx.x - r0 * wide;
   typedef typename Pack<T, VEC>::type raw;
   const int heads = a.heads[0] + a.heads[1], rows = n * heads;
   const int before = a.offset / VEC;
-  // units in the order of their places (neighbouring lanes, neighbouring addresses); the half layout's skip the second entries
+  // units in the order of their places (neighbouring lanes, neighbouring addresses); where a unit is two accesses, the second's place is skipped
   auto turns = [&](int u) { return u >= before && u - before < turning; };
   raw x, y;
   T* dst;
   int tok;
   auto fetch = [&](int u, int row) {
-    const int at = HALF && u - before >= turning ? u * VEC + pairs : u * VEC;
+    int at = TWO && u - before >= turning ? u * VEC + pairs : u * VEC;
+    if (TWO && !HALF && turns(u)) at += u - before;
     tok = row / heads;
     const int hh = row - tok * heads, which = hh >= a.heads[0], h = which ? hh - a.heads[0] : hh;
     const T* src = static_cast<const T*>(a.src[which]) + (t0 + tok) * a.s_tok[which] + h * a.s_head[which] + at;
     dst = static_cast<T*>(a.dst[which]) + (t0 + tok) * a.d_tok[which] + h * a.d_head[which] + at;
     x = *reinterpret_cast<const raw*>(src);
-    if (HALF && turns(u)) y = *reinterpret_cast<const raw*>(src + pairs);
+    if (TWO && turns(u)) y = *reinterpret_cast<const raw*>(src + apart);
   };
   // The first entries are on their way while the table is made: 65536 tokens x 40 heads of 128 bf16, half of each interleaved, 285 ->
   // 238 us; 25120 x 24 heads of 64 fp32 55 -> 49; all of each, half layout, 236 (two rows at a time, behind the table) -> 242.
@@ -98,10 +102,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
       if (u != u0 || row != r0) fetch(u, row);
       raw* const out = reinterpret_cast<raw*>(dst);
       if (!turns(u)) { *out = x; continue; }
-      constexpr int P = HALF ? VEC : VEC / 2;      // pairs of a unit
+      constexpr int P = TWO ? VEC : VEC / 2;       // pairs of a unit
       const float* c = cosines + tok * pairs + (u - before) * P;
       const float* s = sines + tok * pairs + (u - before) * P;
-      if constexpr (HALF) {
+      if constexpr (TWO) {
         raw ox, oy;
         if constexpr (VEC == 1) {
           ox = (T)((float)x * c[0] - (float)y * s[0]);
@@ -114,8 +118,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
           }
         }
         *out = ox;
-        *reinterpret_cast<raw*>(dst + pairs) = oy;
-      } else if constexpr (VEC >= 2) {
+        *reinterpret_cast<raw*>(dst + apart) = oy;
+      } else {
         raw o;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
@@ -131,7 +135,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
 template <class T, int VEC>
 void launch(const RotaryArgs& a, bool half, unsigned blocks, size_t lds, hipStream_t stream) {
   if (half) hipLaunchKernelGGL((rotary_kernel<T, VEC, true>), dim3(blocks), dim3(256), lds, stream, a);
-  else if constexpr (VEC >= 2) hipLaunchKernelGGL((rotary_kernel<T, VEC, false>), dim3(blocks), dim3(256), lds, stream, a);
+  else hipLaunchKernelGGL((rotary_kernel<T, VEC, false>), dim3(blocks), dim3(256), lds, stream, a);
 }
 
 template <class T>
@@ -160,8 +164,9 @@ extern "C" int ac_rotary(const ac_rotary_args* r, void* stream) {
   AC_REQUIRE(((uintptr_t)r->frequencies & 7) == 0 && ((uintptr_t)r->positions & (r->positions64 ? 7 : 3)) == 0, "ac_rotary: misaligned positions or frequencies");
   const int size = r->type == AC_F32 ? 4 : 2;
   const bool half = r->layout == AC_ROTARY_HALF;
+  AC_REQUIRE(half || r->offset % 2 == 0, "ac_rotary: interleaved pairs need an even offset");
   RotaryArgs a;
-  // the widest access that every address allows: 16 bytes, two elements or (half layout only) one
+  // the widest access that every address allows: 16 bytes, two elements or one (the stride of an axis of one addresses nothing)
   int64_t all = half ? (int64_t)r->part / 2 : r->part;
   all |= r->offset | r->dim;
   for (int i = 0; i < 2; ++i) {
@@ -171,11 +176,11 @@ extern "C" int ac_rotary(const ac_rotary_args* r, void* stream) {
     AC_REQUIRE(r->src[i] && r->dst[i], "ac_rotary: null pointer");
     AC_REQUIRE(((uintptr_t)r->src[i] | (uintptr_t)r->dst[i]) % size == 0, "ac_rotary: misaligned tensor");
     all |= (int64_t)((uintptr_t)r->src[i] / size) | (int64_t)((uintptr_t)r->dst[i] / size);
-    all |= r->src_token[i] | r->src_head[i] | r->dst_token[i] | r->dst_head[i];
+    if (r->tokens > 1) all |= r->src_token[i] | r->dst_token[i];
+    if (r->heads[i] > 1) all |= r->src_head[i] | r->dst_head[i];
   }
   const int wide = 16 / size;
   const int vec = all % wide == 0 ? wide : all % 2 == 0 ? 2 : 1;
-  AC_REQUIRE(half || vec >= 2, "ac_rotary: interleaved pairs need an even offset, head dim, strides and addresses");
   a.positions = r->positions; a.pos_axis = r->position_axis; a.pos64 = r->positions64; a.freq = r->frequencies;
   a.tokens = r->tokens; a.dim = r->dim; a.part = r->part; a.offset = r->offset; a.axes = r->axes;
   a.amplitude = r->amplitude; a.inverse = r->inverse;

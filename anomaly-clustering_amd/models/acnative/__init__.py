@@ -1011,7 +1011,8 @@ def rotary_frequencies(part, base=10000.0, axes=1, factor=1.0, original=None, lo
 
 def rotary(q, k, positions, frequencies, layout="half", offset=0, amplitude=1.0, inverse=False, out_q=None, out_k=None):
     """Rotary positions of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (or None): pair i of a head turns by
-    position * frequencies[i] in entries offset .. offset + part, the rest is copied (include/ac_hip.h ac_rotary).
+    position * frequencies[i] in entries offset .. offset + part, the rest is copied (include/ac_hip.h ac_rotary).  Interleaved
+    pairs need an even offset.
 
     positions: int32 / int64 [tokens] or [axes, tokens]; frequencies: fp64 [axes, part / 2 / axes] (or [part / 2]) on the
     device (rotary_frequencies).  inverse=True turns back by the same angles (the transpose of the map: its gradient).

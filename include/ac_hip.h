@@ -340,7 +340,7 @@ int ac_cluster_scores(const int32_t* labels_true, const int32_t* labels_pred, in
 
 /* Rotary positions: pair i of each head turns by angle = position * frequencies[i]: (a, b) -> amplitude * (a cos - b sin,
  * b cos + a sin); inverse != 0 turns back (the transpose of the map: what a gradient needs).  Entries offset .. offset + part
- * of a head turn, the others are copied.  frequencies: fp64 [part / 2], radians per position; pairs of axis x, x = i / (part / 2
+ * of a head turn (interleaved: an even offset), the others are copied.  frequencies: fp64 [part / 2], radians per position; pairs of axis x, x = i / (part / 2
  * / axes), use the positions at x * position_axis.  Positions are int32, or int64 with positions64 != 0, and may be negative;
  * angles are formed in fp64.  src / dst / heads [0] is q, [1] is k (heads[1] = 0: q alone).  dst may be src with the same
  * strides, and must not overlap it otherwise. */

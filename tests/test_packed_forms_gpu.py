@@ -1,0 +1,57 @@
+"""GPU parity: forms and plans of the packed-sequence operators that test_packed_gpu.py does not reach (its bounds hold here too)."""
+import math
+
+import pytest
+import torch
+
+import acnative
+from oracle import packed as opacked
+from test_packed_gpu import E, KINDS, _check_attention, _randn, _run, _starts, _u
+
+pytestmark = pytest.mark.gpu
+
+
+def _check_rotary(got, x, pos, freq, layout, offset, amplitude, kind, inverse=False):
+    ref, size = opacked.rotary(x, pos, freq, layout, offset, amplitude, inverse)
+    tol = _u(kind) * ref.abs() + (2.0 ** -22 + 4 * E) * size + (2.0 ** -25 if kind == "fp16" else 0.0)
+    assert ((got.cpu().double() - ref).abs() <= tol).all()
+
+
+# ----------------------------------------------------------------------------------------------------------- rotary
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("D,part,offset", [(48, 48, 0), (80, 24, 8), (37, 20, 6), (3, 2, 0), (300, 10, 286)])
+def test_rotary_interleaved_on_odd_strides(dev, kind, D, part, offset):
+    """Heads that start at odd entries, odd head sizes: a slice of [tokens, heads, dim + 3], turned beside itself and in place."""
+    T, H, G = 19, 4, 2
+    base = _randn((T + 1, H + G + 1, D + 3), D, kind)
+    x, xk = base[1:, 1:H + 1, 3:], base[1:, H + 1:, 3:]
+    pos = torch.randint(0, 100000, (T,), generator=torch.Generator().manual_seed(1), dtype=torch.int32)
+    freq = acnative.rotary_frequencies(part)
+    d = base.to(dev)
+    q, k = d[1:, 1:H + 1, 3:], d[1:, H + 1:, 3:]
+    args = (pos.to(dev), freq.to(dev))
+    for a, b in zip(acnative.rotary(q, k, *args, layout="interleaved", offset=offset, amplitude=0.75), (x, xk)):
+        _check_rotary(a, b, pos, freq, "interleaved", offset, 0.75, kind)
+    acnative.rotary(q, k, *args, layout="interleaved", offset=offset, amplitude=0.75, out_q=q, out_k=k)
+    _check_rotary(q, x, pos, freq, "interleaved", offset, 0.75, kind)
+    _check_rotary(k, xk, pos, freq, "interleaved", offset, 0.75, kind)
+    rest = torch.ones(base.shape, dtype=torch.bool)
+    rest[1:, 1:, 3 + offset:3 + offset + part] = False
+    assert torch.equal(d.cpu()[rest], base[rest])
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_strides_of_axes_of_one(dev, layout):
+    """A tensor of one token or one head may carry any stride for that axis."""
+    base = _randn((3, 5, 64), 1, "bf16")
+    d = base.to(dev)
+    freq = acnative.rotary_frequencies(64)
+    pos = torch.tensor([123, 7, 99], dtype=torch.int32)
+    one = d.as_strided((1, 5, 64), (321, 64, 1))
+    out = torch.zeros(400, dtype=torch.bfloat16, device=dev).as_strided((1, 5, 64), (333, 64, 1))
+    acnative.rotary(one, None, pos[:1].to(dev), freq.to(dev), layout=layout, out_q=out)
+    _check_rotary(out, base[:1], pos[:1], freq, layout, 0, 1.0, "bf16")
+    head = d.as_strided((3, 1, 64), (320, 7, 1))
+    got = acnative.rotary(head, head, pos.to(dev), freq.to(dev), layout=layout)
+    for y in got:
+        _check_rotary(y, base[:, :1], pos, freq, layout, 0, 1.0, "bf16")
