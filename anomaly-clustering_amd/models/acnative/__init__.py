@@ -12,6 +12,7 @@ import struct
 import threading
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("AC_LIB") or os.path.join(_HERE, "libac_hip.so")   # AC_LIB: diagnostic builds only
@@ -905,6 +906,13 @@ def _no_cpu(t, name):
     raise RuntimeError("%s must be a tensor on the HIP device (got %s); the MI355X path has no CPU fallback" % (name, getattr(t, "device", type(t))))
 
 
+def _refuse_gradient(t, name, text):
+    """A gradient that would have to pass through `t` would be lost: reverse mode, or a tangent of forward mode (such a tensor
+    requires none).  Called where either can be: `t.requires_grad or _forward_ad._current_level >= 0`."""
+    if (t.requires_grad and torch.is_grad_enabled()) or _forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError("%s requires a gradient: %s" % (name, text))
+
+
 def _heads(t, name, like=None):
     """Checks a [tokens, heads, dim] device tensor with neighbouring entries, of `like`'s (dtype, device, dim); -> shape, strides."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -914,8 +922,8 @@ def _heads(t, name, like=None):
         raise ValueError("%s must be [tokens, heads, dim], got %s" % (name, tuple(shape)))
     if strides[2] != 1 and shape[2] > 1:
         raise ValueError("%s: the entries of a head must be neighbours (stride 1), got stride %d" % (name, strides[2]))
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("%s requires a gradient: this operator has no backward pass (use torch.no_grad() or detach())" % name)
+    if t.requires_grad or _forward_ad._current_level >= 0:
+        _refuse_gradient(t, name, "this operator has no backward pass (use torch.no_grad() or detach())")
     if like is None:
         if t.dtype not in _TYPES:
             raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
@@ -937,6 +945,8 @@ def _whole(t, dtypes, name, device):
         raise TypeError("%s must be %s, got %s" % (name, " or ".join(str(d) for d in dtypes), t.dtype))
     if not t.is_contiguous():
         raise ValueError("%s must be contiguous" % name)
+    if t.requires_grad or _forward_ad._current_level >= 0:
+        _refuse_gradient(t, name, "this operator has none for it (use torch.no_grad() or detach())")
     return t
 
 
@@ -1169,8 +1179,8 @@ def _rows(t, name, like=None):
     shape = t.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError("%s must be [..., width], got %s" % (name, tuple(shape)))
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("%s requires a gradient: this operator records no graph (layer_norm_backward has the gradients)" % name)
+    if t.requires_grad or _forward_ad._current_level >= 0:
+        _refuse_gradient(t, name, "this operator records no graph (layer_norm_backward has the gradients)")
     if like is None:
         if t.dtype not in _TYPES:
             raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
@@ -1188,8 +1198,8 @@ def _norm_vector(t, name, x, dtype, device, width):
         raise ValueError("%s must be [%d], got %s" % (name, width, tuple(t.shape)))
     if t.dtype != dtype and t.dtype != torch.float32:
         raise TypeError("%s must be %s or float32, got %s" % (name, dtype, t.dtype))
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("%s requires a gradient: this operator records no graph (layer_norm_backward has the gradients)" % name)
+    if t.requires_grad or _forward_ad._current_level >= 0:
+        _refuse_gradient(t, name, "this operator records no graph (layer_norm_backward has the gradients)")
     return t if t.stride(0) == 1 or width == 1 else t.contiguous()
 
 

@@ -55,3 +55,43 @@ def test_rotary_strides_of_axes_of_one(dev, layout):
     got = acnative.rotary(head, head, pos.to(dev), freq.to(dev), layout=layout)
     for y in got:
         _check_rotary(y, base[:, :1], pos, freq, layout, 0, 1.0, "bf16")
+
+
+# ------------------------------------------------------------------------------------- gradients that would be lost
+def test_a_tangent_is_refused_like_a_gradient(dev):
+    """Forward-mode differentiation: a dual tensor does not require a gradient, and its tangent would be dropped."""
+    x = torch.ones(8, 4, 64, device=dev)
+    starts = torch.tensor([0, 8], dtype=torch.int32, device=dev)
+    freq, pos = acnative.rotary_frequencies(64, device=dev), torch.zeros(8, dtype=torch.int32, device=dev)
+    w = torch.ones(64, device=dev)
+    mean = torch.zeros(8, 4, device=dev)
+    fwd = torch.autograd.forward_ad
+    calls = (lambda t: acnative.rotary(t, None, pos, freq), lambda t: acnative.rotary(x, t, pos, freq), lambda t: acnative.rotary(x, None, pos, freq, out_q=t),
+             lambda t: acnative.attention_packed(t, x, x, starts), lambda t: acnative.attention_packed(x, t, x, starts),
+             lambda t: acnative.attention_packed(x, x, t, starts), lambda t: acnative.layer_norm(t), lambda t: acnative.layer_norm(x, out=t),
+             lambda t: acnative.layer_norm_backward(t, x, None, mean, mean), lambda t: acnative.layer_norm_backward(x, t, None, mean, mean))
+    vectors = (lambda t: acnative.layer_norm(x, t), lambda t: acnative.layer_norm(x, w, t), lambda t: acnative.layer_norm_backward(x, x, t, mean, mean))
+    with fwd.dual_level():
+        for call in calls:
+            with pytest.raises(RuntimeError, match="gradient"):
+                call(fwd.make_dual(torch.ones_like(x), torch.ones_like(x)))
+            call(torch.ones_like(x))                              # without a tangent: fine inside a level too
+        for call in vectors:
+            with pytest.raises(RuntimeError, match="gradient"):
+                call(fwd.make_dual(w.clone(), torch.ones_like(w)))
+        with pytest.raises(RuntimeError, match="gradient"):
+            acnative.rotary(x, None, pos, fwd.make_dual(freq.clone(), torch.ones_like(freq)))
+
+
+def test_frequencies_and_statistics_that_require_a_gradient_are_refused(dev):
+    x = torch.ones(8, 4, 64, device=dev)
+    pos, freq = torch.zeros(8, dtype=torch.int32, device=dev), acnative.rotary_frequencies(64, device=dev)
+    stat = torch.ones(8, 4, device=dev)
+    learned = freq.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="gradient"):
+        acnative.rotary(x, None, pos, learned)
+    for a, b in ((stat.clone().requires_grad_(), stat), (stat, stat.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="gradient"):
+            acnative.layer_norm_backward(x, x, None, a, b)
+    with torch.no_grad():
+        assert acnative.rotary(x, None, pos, learned).shape == x.shape
