@@ -966,7 +966,7 @@ def _disjoint(a, b):
 
 
 def _apart(a, b):
-    """No entry of `a` is one of `b`: their spans do not meet, or both are head ranges of the same rows (slices of one buffer)."""
+    """No entry of `a` is one of `b`: their spans do not meet, or both are ranges of the same rows (heads or columns of one buffer)."""
     if _disjoint(a, b):
         return True
     if a.stride(0) != b.stride(0) or a.element_size() != b.element_size():
@@ -1227,8 +1227,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, want_stats=False):
         if to.data_ptr() != out.data_ptr():
             raise ValueError("out: its axes must fold into rows of one stride, entries neighbours (strides %s)" % (tuple(out.stride()),))
         _writable(out, "out")
-        for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
-            if t is not None and not _disjoint(out, t) and not (t is x and _same_view(out, x)):
+        if not _apart(to, rows) and not _same_view(out, x):
+            raise ValueError("out overlaps x")
+        for t, name in ((weight, "weight"), (bias, "bias")):
+            if t is not None and not _disjoint(out, t):
                 raise ValueError("out overlaps %s" % name)
         out_row = to.stride(0)
     mean = rstd = None

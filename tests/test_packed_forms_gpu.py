@@ -95,3 +95,21 @@ def test_frequencies_and_statistics_that_require_a_gradient_are_refused(dev):
             acnative.layer_norm_backward(x, x, None, a, b)
     with torch.no_grad():
         assert acnative.rotary(x, None, pos, learned).shape == x.shape
+
+
+# ------------------------------------------------------------------------------------------------ norm beside its input
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_layer_norm_into_the_other_columns_of_its_rows(dev, kind):
+    """x and out as column ranges of one buffer: their spans cross, their entries do not."""
+    T, C = 33, 96
+    both = torch.cat([_randn((T, C), 1, kind), torch.full((T, C), 7.0, dtype=KINDS[kind])], 1).to(dev)
+    x, out = both[:, :C], both[:, C:]
+    w, b = _randn((C,), 2, kind).to(dev), _randn((C,), 3, kind).to(dev)
+    want = acnative.layer_norm(x.contiguous(), w, b)
+    assert acnative.layer_norm(x, w, b, out=out) is out
+    assert torch.equal(out, want) and torch.equal(x.cpu(), _randn((T, C), 1, kind))
+    three = both.view(3, 11, 2 * C)
+    assert torch.equal(acnative.layer_norm(three[..., C:], w, b, out=three[..., :C]).reshape(T, C), acnative.layer_norm(want, w, b))
+    for bad in (both[:, 1:C + 1], both[:, C - 1:2 * C - 1]):
+        with pytest.raises(ValueError, match="overlaps"):
+            acnative.layer_norm(both[:, :C], w, b, out=bad)
