@@ -13,6 +13,7 @@ import threading
 
 import torch
 from torch.autograd import forward_ad as _forward_ad
+from torch.autograd.graph import increment_version as _written      # after writing into a caller's tensor: a graph that saved it has to notice
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("AC_LIB") or os.path.join(_HERE, "libac_hip.so")   # AC_LIB: diagnostic builds only
@@ -1053,6 +1054,7 @@ def rotary(q, k, positions, frequencies, layout="half", offset=0, amplitude=1.0,
     axes = fshape[0] if len(fshape) == 2 else 1
     if pshape != (axes, tokens) and not (axes == 1 and pshape == (tokens,)):
         raise ValueError("positions must be [%d, %d]%s, got %s" % (axes, tokens, " or [%d]" % tokens if axes == 1 else "", tuple(pshape)))
+    given = [t for t in (out_q, out_k) if t is not None]
     if out_q is None:
         out_q = _fresh(q)
         os = (heads * dim, dim)
@@ -1072,6 +1074,8 @@ def rotary(q, k, positions, frequencies, layout="half", offset=0, amplitude=1.0,
         q.data_ptr(), kp, out_q.data_ptr(), out_k.data_ptr() if k is not None else 0, qs[0], ks[0], qs[1], ks[1], os[0], kos[0], os[1], kos[1],
         heads, kv_heads, positions.data_ptr(), tokens, positions.dtype == torch.int64, frequencies.data_ptr(), tokens, _TYPES[dtype],
         _LAYOUTS[layout], dim, 2 * pairs, offset, axes, bool(inverse), amplitude))
+    if given:
+        _written(given)
     return out_q if k is None else (out_q, out_k)
 
 
@@ -1158,6 +1162,8 @@ def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, c
     # of its own for every call: two graphs captured on one stream must not share the parts of a split key axis
     ws = q.new_empty(n, dtype=torch.uint8) if n else None
     _launch(device, handle.ac_attention_packed, args, ws.data_ptr() if n else None, n)
+    if not clear:
+        _written(out)
     return (out, sums) if want_sums else out
 
 
@@ -1219,7 +1225,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, want_stats=False):
         kind = weight.dtype
         if bias is not None and bias.dtype != kind:
             raise TypeError("weight is %s, but bias is %s" % (kind, bias.dtype))
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = _fresh(x)
         out_row, to = width, out
     else:
@@ -1240,6 +1247,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, want_stats=False):
         rows.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(), to.data_ptr(), 0, 0, 0, 0,
         mean.data_ptr() if want_stats else 0, rstd.data_ptr() if want_stats else 0, rows.stride(0) if count > 1 else width,
         out_row if count > 1 else width, 0, 0, count, width, _TYPES[dtype], _TYPES[kind], eps))
+    if not fresh:
+        _written(out)
     return (out, mean, rstd) if want_stats else out
 
 

@@ -113,3 +113,21 @@ def test_layer_norm_into_the_other_columns_of_its_rows(dev, kind):
     for bad in (both[:, 1:C + 1], both[:, C - 1:2 * C - 1]):
         with pytest.raises(ValueError, match="overlaps"):
             acnative.layer_norm(both[:, :C], w, b, out=bad)
+
+
+def test_writing_into_a_tensor_is_seen_by_autograd(dev):
+    """A tensor that a graph has saved and an operator then writes into: backward has to refuse, not to use the new values."""
+    pos, freq = torch.arange(8, dtype=torch.int32, device=dev), acnative.rotary_frequencies(64, device=dev)
+    starts = torch.tensor([0, 8], dtype=torch.int32, device=dev)
+    other = torch.ones(8, 4, 64, device=dev)
+    for write in (lambda t: acnative.rotary(t, None, pos, freq, out_q=t), lambda t: acnative.rotary(other, t, pos, freq, out_k=t),
+                  lambda t: acnative.layer_norm(t, out=t), lambda t: acnative.attention_packed(other, other, other, starts, out=t)):
+        leaf = torch.ones(8, 4, 64, device=dev, requires_grad=True)
+        y = leaf * 2
+        z = (y * y).sum()
+        write(y.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward()
+    with torch.inference_mode():
+        t = torch.ones(8, 4, 64, device=dev)
+        assert acnative.rotary(t, None, pos, freq, out_q=t) is t
