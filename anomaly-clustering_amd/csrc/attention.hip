@@ -37,7 +37,7 @@ struct AttArgs {
   uint32_t q_keep, q_flip;           // bits of q that stay, and that turn: a negative scale negates q, a zero one clears it
   int clear;                         // rows before the first and behind the last sequence: 1 zero in out, 2 -inf in sums
   int pairs, replicas, together, tiles, splits, chunk;    // the grid (launch())
-  float* part_o; float* part_ml;     // partial results of a split key axis
+  float* part_o; float* part_ml;     // a split key axis: each part's weighted mean, and its maximum and sum
 };
 
 // ---- the three types: a 16-byte fragment, its products, and P
@@ -174,7 +174,12 @@ struct Shape {
 };
 
 // Rows [first, last) of a wave once more, key by key, over the keys that each sees alone: where values that some row does not see
-// are infinite or NaN.  Lane -> key for the scores, -> entries of the head for the sum.  Not made to be fast.
+// are infinite or NaN, and where a sum of finite scores and weights came out infinite or NaN.  That happens to finite values too:
+// the sums below weigh them up to 2^8 (rescale()), n keys add up, and from FLT_MAX / (2^8 n) on they leave the range though their
+// weighted mean does not; and to an infinite value whose weight is 0 in the tensor's type (fp16: under 2^-25) and not in fp32.
+// Here weights are at most 2^-K with 2^K > n, exactly scaled, and stay fp32, so that no finite value overflows.  Lane -> key for
+// the scores, -> entries of the head for the sum.  Not made to be fast: 4096 causal tokens, 16 / 4 heads of 128 bf16, every row done
+// again 68 ms (0.12 without).
 template <class T, int DMAX>
 __device__ inline void again(const AttArgs& a, int split, int begin, int end, int q0, int nq, int k0, int nk, int kvh, int first, int last, int lane) {
   constexpr int ND = (DMAX + 63) / 64;
@@ -186,6 +191,8 @@ __device__ inline void again(const AttArgs& a, int split, int begin, int end, in
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = 0.f;
     const float c = a.q_keep ? (a.q_flip ? -a.c_log2 : a.c_log2) : 0.f;
+    const int bits = 32 - __builtin_clz(max(seen - begin, 1));               // K
+    const float down = __builtin_bit_cast(float, (uint32_t)(127 - bits) << 23), up = __builtin_bit_cast(float, (uint32_t)(127 + bits) << 23);
     for (int key = begin; key < seen; key += 64) {
       const int n = min(64, seen - key);
       float s = -__builtin_inff();
@@ -200,7 +207,7 @@ __device__ inline void again(const AttArgs& a, int split, int begin, int end, in
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] *= corr;
       for (int j = 0; j < n; ++j) {
-        const float w = __shfl(p, j, 64);
+        const float w = __shfl(p, j, 64) * down;
         const T* v = static_cast<const T*>(a.v) + (int64_t)(k0 + key + j) * a.v_tok + (int64_t)kvh * a.v_head;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -209,14 +216,14 @@ __device__ inline void again(const AttArgs& a, int split, int begin, int end, in
       m = m_new;
     }
     const size_t at = (size_t)(q0 + i) * a.heads + hh;
+    const float inv = l == 0.f ? 0.f : 1.0f / l * up;
     if (a.splits > 1) {
       const size_t part = (size_t)split * a.tokens_q * a.heads + at;
       if (lane == 0) { a.part_ml[2 * part] = m; a.part_ml[2 * part + 1] = l; }
 #pragma unroll
       for (int d = 0; d < ND; ++d)
-        if (lane + 64 * d < a.dim) a.part_o[part * a.dim + lane + 64 * d] = o[d];
+        if (lane + 64 * d < a.dim) a.part_o[part * a.dim + lane + 64 * d] = o[d] * inv;
     } else {
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
       T* out = static_cast<T*>(a.out) + (int64_t)(q0 + i) * a.o_tok + (int64_t)hh * a.o_head;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
@@ -224,6 +231,27 @@ __device__ inline void again(const AttArgs& a, int split, int begin, int end, in
       if (a.sums && lane == 0) a.sums[at] = l == 0.f ? -__builtin_inff() : 0.69314718055994530942f * (m + __builtin_amdgcn_logf(l));
     }
   }
+}
+
+// Infinite or NaN outputs of rows whose sums are numbers: do the rows have to be done again?  Not where the values that they see hold
+// a NaN, or an infinity that passes as it is: the outputs then are what they should be (and repeating them would take a hundred
+// times as long as the rest of the call).  Lane -> column.
+template <class T, bool THIRDS>
+__device__ inline bool unexplained(const AttArgs& a, int begin, int end, int nq, int k0, int nk, int kvh, int last, int lane) {
+  bool nan = false, inf = false;
+  const int seen = min(end, a.causal ? min(max((last - 1) / a.group + nk - nq + 1, 0), nk) : nk);
+  for (int d = lane; d < a.dim; d += 64) {
+    const T* v = static_cast<const T*>(a.v) + (int64_t)(k0 + begin) * a.v_tok + (int64_t)kvh * a.v_head + d;
+#pragma unroll 4
+    for (int key = begin; key < seen; ++key, v += a.v_tok) {
+      const float x = (float)*v;
+      nan |= x != x;
+      inf |= __builtin_fabsf(x) == __builtin_inff();
+    }
+  }
+  // an infinity has no thirds, and fp16 may have rounded its weight to 0
+  if (__builtin_amdgcn_ballot_w64(inf)) return THIRDS || __is_same(T, _Float16);
+  return __builtin_amdgcn_ballot_w64(nan) == 0;
 }
 
 template <class T, int NS, int NQ, int WQ, int WK, int KB>
@@ -703,17 +731,25 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
           }
       }
     }
-    if constexpr (G::SPLIT) {                      // NaN: there may be an infinity behind it, which the thirds cannot hold
-      bool nan = false;
+    // Outputs that are not finite: again(), unless the values explain them.  A sum that is NaN says that a score was; thirds make one of
+    // an infinite score, the others are right
+    bool not_finite = false;
+    if (wk == 0) {
+      bool odd = false, sum_odd = false;
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
-        nan |= l_run[b] != l_run[b];
+        const bool there = wave_row + 32 * b + r < rows, number = l_run[b] == l_run[b];
+        float part[4] = {0.f, 0.f, 0.f, 0.f};      // NaN if an entry is not finite
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) nan |= o[b][d][i] != o[b][d][i];
+          for (int i = 0; i < 16; ++i) part[i & 3] = __builtin_fmaf(o[b][d][i], 0.f, part[i & 3]);
+        const float zero = (part[0] + part[1]) + (part[2] + part[3]);
+        odd |= there && number && zero != zero;
+        sum_odd |= there && !number;
       }
-      if (__builtin_amdgcn_ballot_w64(nan)) odd_values = true;
+      not_finite = __builtin_amdgcn_ballot_w64(odd) != 0;
+      if (G::SPLIT && __builtin_amdgcn_ballot_w64(sum_odd)) odd_values = true;
     }
     if constexpr (WK > 1) {
       __syncthreads();
@@ -724,14 +760,13 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
       __syncthreads();
       odd_values = *flag != 0;
     }
-    if (wk == 0 && odd_values) {
-      again<T, DB * 32>(a, split, split_begin, split_end, q0, nq, k0, nk, kvh, wave_row, min(wave_row + 32 * NQ, rows), lane);
-    } else if (wk == 0) {
+    if (wk == 0) {
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
         const int row = wave_row + 32 * b + r;
         if (row >= rows) continue;
         const int i = row / a.group, hh = kvh * a.group + row - i * a.group;
+        const float inv = l_run[b] == 0.f ? 0.f : 1.0f / l_run[b];
         if (a.splits > 1) {
           const size_t at = (size_t)split * a.tokens_q * a.heads + (size_t)(q0 + i) * a.heads + hh;
           float* dst = a.part_o + at * a.dim;
@@ -744,10 +779,9 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int e = 32 * d + 8 * j + 4 * h;
-              if (e < a.dim) *reinterpret_cast<f32x4*>(dst + e) = f32x4{o[b][d][4 * j], o[b][d][4 * j + 1], o[b][d][4 * j + 2], o[b][d][4 * j + 3]};
+              if (e < a.dim) *reinterpret_cast<f32x4*>(dst + e) = f32x4{o[b][d][4 * j] * inv, o[b][d][4 * j + 1] * inv, o[b][d][4 * j + 2] * inv, o[b][d][4 * j + 3] * inv};
             }
         } else {
-          const float inv = l_run[b] == 0.f ? 0.f : 1.0f / l_run[b];
           T* dst = static_cast<T*>(a.out) + (int64_t)(q0 + i) * a.o_tok + (int64_t)hh * a.o_head;
 #pragma unroll
           for (int d = 0; d < DB; ++d)
@@ -764,6 +798,13 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
             a.sums[(size_t)(q0 + i) * a.heads + hh] = l_run[b] == 0.f ? -__builtin_inff() : 0.69314718055994530942f * (m_run[b] + __builtin_amdgcn_logf(l_run[b]));
         }
       }
+    }
+    // (behind the normal output, which again() overwrites: in front of it the scan's scalar registers cost 2 % of the whole)
+    if (wk == 0 && (odd_values || not_finite)) {
+      const int last = min(wave_row + 32 * NQ, rows);
+      wait_transfers<0>();
+      if (odd_values || unexplained<T, G::SPLIT>(a, split_begin, split_end, nq, k0, nk, kvh, last, lane))
+        again<T, DB * 32>(a, split, split_begin, split_end, q0, nq, k0, nk, kvh, wave_row, last, lane);
     }
     __syncthreads();                 // the next tile's transfers overwrite what these waves may still read
   }
@@ -800,9 +841,10 @@ __global__ __launch_bounds__(256) void join_kernel(const AttArgs a) {
     m = ml[0];
     l = ml[1];
   }
-  const float top = wave_max(m), w = lane < parts ? __builtin_amdgcn_exp2f(m - top) : 0.f;
-  l = wave_sum(l * w);
-  if (tid < 64) weight[tid] = w;
+  // the parts hold means: their weights add up to 1, so what is finite stays so
+  const float top = wave_max(m), w = lane < parts ? l * __builtin_amdgcn_exp2f(m - top) : 0.f;
+  l = wave_sum(w);
+  if (tid < 64) weight[tid] = l == 0.f ? 0.f : w / l;
   __syncthreads();
   const int grp = tid >> 5, e = (tid & 31) * 4;
   f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
@@ -825,8 +867,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttArgs a) {
     float x = 0.f;
 #pragma unroll
     for (int g = 0; g < 8; ++g) x += all[g][tid];
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    static_cast<T*>(a.out)[(int64_t)token * a.o_tok + (int64_t)hh * a.o_head + tid] = (T)(x * inv);
+    static_cast<T*>(a.out)[(int64_t)token * a.o_tok + (int64_t)hh * a.o_head + tid] = (T)x;
   }
   if (a.sums && tid == 0) a.sums[row] = l == 0.f ? -__builtin_inff() : 0.69314718055994530942f * (top + __builtin_amdgcn_logf(l));
 }

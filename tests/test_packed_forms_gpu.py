@@ -131,3 +131,62 @@ def test_writing_into_a_tensor_is_seen_by_autograd(dev):
     with torch.inference_mode():
         t = torch.ones(8, 4, 64, device=dev)
         assert acnative.rotary(t, None, pos, freq, out_q=t) is t
+
+
+# --------------------------------------------------------------------------- attention on values at the ends of a type
+def _lagging(n, keys, H, G, D, kind, seed):
+    """q and k whose first 32 keys score about 0 and the later ones up to 2^7.5 times their weight: the running maximum stays."""
+    q, k = torch.zeros(n, H, D), torch.zeros(keys, G, D)
+    q[..., 0] = 1.0
+    k[:, :, 0] = 7.4 * math.log(2.0) * D ** 0.5 * (0.9 + 0.1 * torch.rand(keys, G, generator=torch.Generator().manual_seed(seed)))
+    k[:32, :, 0] = 0.01
+    q[..., 1:], k[..., 1:] = 0.05 * _randn((n, H, D - 1), seed, "fp32"), 0.05 * _randn((keys, G, D - 1), seed + 1, "fp32")
+    return q.to(KINDS[kind]), k.to(KINDS[kind])
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("H,G,D,queries,keys,causal", [(2, 2, 64, [300], [300], False), (2, 1, 128, [200, 70], [500, 70], True), (8, 2, 64, [1, 1], [3000, 700], False),
+                                                       (2, 2, 80, [150], [150], True), (4, 1, 128, [1, 3], [5000, 64], True)])
+def test_attention_of_values_near_the_largest(dev, kind, H, G, D, queries, keys, causal):
+    """Finite values whose weighted sum leaves the type's range where their weighted mean does not."""
+    sq, sk = _starts(queries), _starts(keys)
+    q, k = _lagging(int(sq[-1]), int(sk[-1]), H, G, D, kind, D)
+    v = (_randn((int(sk[-1]), G, D), 9, "fp32").clamp(-4, 4) * 8e37).to(KINDS[kind])
+    ref = opacked.attention(q, k, v, sq, sk, causal)
+    got, sums = acnative.attention_packed(q.to(dev), k.to(dev), v.to(dev), sq.to(dev), sk.to(dev), max_q=max(queries), max_k=max(keys), causal=causal,
+                                          want_sums=True)
+    assert torch.isfinite(got).all()
+    _check_attention(got, sums, ref, kind, D, "near the largest")
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("queries,keys", [([90], [90]), ([1], [3000]), ([300, 20], [400, 20])])
+def test_attention_infinite_values_of_small_weight(dev, kind, queries, keys):
+    """An infinite value that a row sees passes however little it weighs: 2^-50 is nothing in fp16, and 0 times infinity would be NaN."""
+    H, D = 2, 64
+    sq, sk = _starts(queries), _starts(keys)
+    q, k, v = torch.zeros(int(sq[-1]), H, D), torch.zeros(int(sk[-1]), H, D), _randn((int(sk[-1]), H, D), 3, kind)
+    q[..., 0] = 1.0
+    k[..., 0] = 0.1 * _randn((int(sk[-1]), H), 4, "fp32")
+    k[40, 0, 0] = -50 * math.log(2.0) * 8.0
+    v[40, 0, 5], v[40, 0, 6] = math.inf, -math.inf
+    q, k = q.to(KINDS[kind]), k.to(KINDS[kind])
+    ref = opacked.attention(q, k, v, sq, sk, False)
+    assert (ref["out"][:queries[0], 0, 5] == math.inf).all() and (ref["out"][:queries[0], 0, 6] == -math.inf).all()
+    got, sums = acnative.attention_packed(q.to(dev), k.to(dev), v.to(dev), sq.to(dev), sk.to(dev), max_q=max(queries), max_k=max(keys), want_sums=True)
+    _check_attention(got, sums, ref, kind, D, "small weight")
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("queries,keys", [([90], [96]), ([1], [3000]), ([300, 20], [416, 32])])
+def test_attention_of_a_bad_value_that_every_row_sees(dev, kind, bad, queries, keys):
+    """It makes its own column of its own head NaN (or infinite) and touches no other."""
+    H, D = 2, 80
+    sq, sk = _starts(queries), _starts(keys)
+    q, k, v = (_randn((n, H, D), i, kind) for i, n in enumerate((int(sq[-1]), int(sk[-1]), int(sk[-1]))))
+    v[17, 1, 70] = bad
+    ref = opacked.attention(q, k, v, sq, sk, False)
+    assert not torch.isfinite(ref["out"][:queries[0], 1, 70]).any() and (~torch.isfinite(ref["out"])).sum() == queries[0]
+    got, sums = acnative.attention_packed(q.to(dev), k.to(dev), v.to(dev), sq.to(dev), sk.to(dev), max_q=max(queries), max_k=max(keys), want_sums=True)
+    _check_attention(got, sums, ref, kind, D, "bad value")
