@@ -57,6 +57,27 @@ def test_rotary_strides_of_axes_of_one(dev, layout):
         _check_rotary(y, base[:, :1], pos, freq, layout, 0, 1.0, "bf16")
 
 
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_turned_back(dev, kind, layout):
+    """inverse=True is the transpose of the map, amplitude included: against the oracle, and <y, R x> = <R^T y, x>."""
+    T, H, G, D, part, offset = 45, 4, 2, 80, 48, 16
+    x, y = _randn((T, H, D), 1, kind), _randn((T, G, D), 2, kind)
+    pos = torch.randint(-5, 4_000_000, (2, T), generator=torch.Generator().manual_seed(3), dtype=torch.int64)
+    freq = acnative.rotary_frequencies(part, 10000.0, axes=2, factor=4.0, original=2048)
+    args = {"layout": layout, "offset": offset, "amplitude": 1.25}
+    got = acnative.rotary(x.to(dev), y.to(dev), pos.to(dev), freq.to(dev), inverse=True, **args)
+    for a, b in zip(got, (x, y)):
+        _check_rotary(a, b, pos, freq, layout, offset, 1.25, kind, inverse=True)
+    if kind == "fp32":
+        y = _randn((T, H, D), 4, kind)
+        turned = acnative.rotary(x.to(dev), None, pos.to(dev), freq.to(dev), **args).cpu().double()
+        back = acnative.rotary(y.to(dev), None, pos.to(dev), freq.to(dev), inverse=True, **args).cpu().double()
+        # each entry of either is off by the bound of _check_rotary: below 2^-21 of the two magnitudes behind it, times 1.25 for the amplitude
+        slack = 2 * 2.0 ** -21 * 1.25 * 2 * (x.double().abs().amax(-1) * y.double().abs().amax(-1)).sum() * D
+        assert abs((y.double() * turned).sum() - (back * x.double()).sum()) <= slack
+
+
 # ------------------------------------------------------------------------------------- gradients that would be lost
 def test_a_tangent_is_refused_like_a_gradient(dev):
     """Forward-mode differentiation: a dual tensor does not require a gradient, and its tangent would be dropped."""
@@ -190,3 +211,77 @@ def test_attention_of_a_bad_value_that_every_row_sees(dev, kind, bad, queries, k
     assert not torch.isfinite(ref["out"][:queries[0], 1, 70]).any() and (~torch.isfinite(ref["out"])).sum() == queries[0]
     got, sums = acnative.attention_packed(q.to(dev), k.to(dev), v.to(dev), sq.to(dev), sk.to(dev), max_q=max(queries), max_k=max(keys), want_sums=True)
     _check_attention(got, sums, ref, kind, D, "bad value")
+
+
+# --------------------------------------------------------------------------------- attention's plans for many rows
+def _plan(dev, kind, heads, kv_heads, D, queries):
+    """The rule of make_plan (csrc/attention.hip) for 16-bit rows: 2: 32 rows and split keys, 1: 128 rows, 0: 256 rows (64 to a wave),
+    3: 128 rows (64 to a wave, two waves)."""
+    cus = torch.cuda.get_device_properties(dev).multi_processor_count
+    rows, pairs, tokens = max(max(queries), -(-sum(queries) // len(queries))) * (heads // kv_heads), len(queries) * kv_heads, sum(queries)
+    if rows <= 32:
+        return 2
+    if kind == "fp32" or D * 2 > 256 or pairs * -(-rows // 256) < 2 * cus:
+        return 1
+    return 3 if D * 2 > 128 and tokens * heads // 256 < 8 * cus else 0
+
+
+def _many(count, top, seed):
+    g = torch.Generator().manual_seed(seed)
+    n = torch.randint(1, top, (count,), generator=g).tolist()
+    n[:14] = [0, 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257]
+    n[20] = 300
+    return n
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("plan,D,heads,kv_heads", [(0, 8, 8, 4), (0, 24, 8, 4), (0, 32, 4, 4), (0, 48, 8, 4), (0, 64, 12, 4), (0, 64, 4, 4),
+                                                   (3, 72, 8, 4), (3, 80, 4, 4), (3, 96, 8, 4), (3, 104, 4, 4), (3, 128, 12, 4), (3, 128, 4, 4)])
+def test_attention_of_many_rows(dev, kind, plan, D, heads, kv_heads):
+    """64 rows a wave: masks over two blocks of rows, shared heads, keys of other lengths, log-sums, ends inside tiles."""
+    queries, keys = _many(70 if heads > kv_heads else 132, 120, D), _many(70 if heads > kv_heads else 132, 160, D + 1)
+    assert _plan(dev, kind, heads, kv_heads, D, queries) == plan
+    _run(dev, kind, heads, kv_heads, D, queries, causal=D % 16 == 0, seed=D)
+    keys[1:14] = [400, 0, 32, 20, 330, 64, 10, 300, 128, 129, 1, 500, 257]
+    _run(dev, kind, heads, kv_heads, D, queries, keys, causal=True, seed=D + 1)
+    if D in (64, 80, 128):
+        _run(dev, kind, heads, kv_heads, D, queries, keys, causal=False, seed=D + 2, qscale=40.0, scale=-0.1, before=3, behind=5)
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("D", [80, 128])
+def test_attention_of_many_rows_of_wide_heads(dev, kind, D):
+    """Heads of more than 128 bytes in blocks of 256 rows: 2^19 rows or more."""
+    g = torch.Generator().manual_seed(D)
+    queries = torch.randint(20, 60, (430,), generator=g).tolist() + [300, 257, 64, 1, 0]
+    assert _plan(dev, kind, 32, 8, D, queries) == 0
+    _run(dev, kind, 32, 8, D, queries, causal=True, seed=D)
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("plan,D", [(0, 64), (0, 40), (3, 72), (3, 128)])
+def test_attention_of_many_rows_what_a_row_does_not_see_cannot_touch_it(dev, kind, plan, D):
+    """Infinities and NaN in keys and values behind a causal row, in the next sequence and in the next head, with 64 rows a wave."""
+    n, H = 150, 8
+    lengths = [n, 40] + _many(68, 60, D)
+    lengths[22] = 200
+    assert _plan(dev, kind, H, H, D, lengths) == plan
+    sq = _starts(lengths, 3)
+    T = int(sq[-1]) + 5
+    q, k, v = (_randn((T, H, D), i, kind) for i in (1, 2, 3))
+    for t in (k, v):
+        t[:3] = math.nan
+        t[int(sq[-1]):] = math.inf
+    v[3 + 100, 0, 5] = math.inf
+    v[3 + 120, 0, 6] = math.nan
+    v[3 + 130, 1, 7] = -math.inf
+    k[3 + 140, 0] = math.nan
+    clean = k.clone()
+    clean[3 + 140, 0] = 0.0
+    ref = opacked.attention(q, clean, v, sq, sq, True)
+    ref["out"][3 + 140:3 + n, 0] = math.nan                        # these rows see the NaN key: NaN throughout
+    out = torch.full((T, H, D), 7.0, dtype=KINDS[kind], device=dev)
+    acnative.attention_packed(q.to(dev), k.to(dev), v.to(dev), sq.to(dev), max_q=max(lengths), max_k=max(lengths), causal=True, out=out)
+    assert (out[:3] == 7.0).all() and (out[int(sq[-1]):] == 7.0).all()
+    inside = slice(3, int(sq[-1]))
+    _check_attention(out[inside], None, {key: x[inside] for key, x in ref.items()}, kind, D, "poisoned")
