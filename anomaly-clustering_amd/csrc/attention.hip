@@ -11,12 +11,17 @@
 //
 // Bounds, and what was reached (16-bit heads unless said otherwise; a large matrix product reaches 1390 TFLOP/s here):
 //   many rows: the products and the exponentials, which share a wave's issue.  A 32x32x16 product takes 32 clocks of the matrix
-//     unit; beside it one wave hides 4 vector instructions, two waves of a SIMD 6.  Heads of 128 (64 rows a wave, one wave a SIMD,
-//     its loop pipelined): 1040 TFLOP/s on a causal prompt of 16384; heads of 64 (two waves a SIMD), where a score has half the
-//     products to its exponential: 920 on 4096 x 4096; images of 1 .. 2305 tokens 630, of which a quarter is rows that do not
-//     fill a tile.  64 rows a wave, because K and V come from LDS: with 32 the reads alone would take as long as the products.
-//   single queries: the bytes of K and V.  64 on 4096 keys each 5.9 TB/s, 16 on 1 .. 16000 keys 4.8 (a copy: 5.2).
-//   fp32: six bf16 products for one (below), 176 .. 204 TFLOP/s, where the fp32 instruction reached 105 .. 140.
+//     unit; four vector instructions beside it add 5 in one wave and 2 with two waves on the SIMD, eight add 19 and 13 (a score
+//     block needs 5.5 to a product with heads of 128, 12 with heads of 64).  Heads of 128 (64 rows a wave, one wave a SIMD,
+//     its loop pipelined): 1020 TFLOP/s on a causal prompt of 16384 (16 / 4 heads), 920 on 8 causal prompts of 4096 (32 / 8); heads
+//     of 64 (two waves a SIMD), where a score has half the products to its exponential: 960 on 8 x 4096 tokens (12 heads); images
+//     of 1 .. 2305 tokens 640, of which a fifth is rows that do not fill a tile.  64 rows a wave, because K and V come from LDS:
+//     with 32 the reads alone would take as long as the products.  Heads of 80: 660 on 3 x 4097, 2305, 3137 tokens (16 heads; 96
+//     output columns, bank conflicts in half of the LDS cycles).
+//   few rows on keys that are there already (up to 512 queries on 900 .. 8077 keys): 250, the grid's bounds leave blocks empty.
+//   single queries: the bytes of K and V.  64 on 4096 keys each 5.7 TB/s, 16 on 1 .. 16000 keys 4.7 (a copy: 5.0); fp32 3.0.
+//   fp32: six bf16 products for one (below), 178 on 32 x 785 tokens, 213 on 8 x 4096 (12 heads of 64), where the fp32 instruction
+//     reached 105 .. 140.
 #include "common.h"
 
 namespace {
@@ -68,8 +73,11 @@ template <> struct Num<float> {
   }
 };
 
-// fp32 on the bf16 products: x = h + m + l, three bf16 values of 8 bits each, exactly (h and m cut off, no rounding, so that no
-// finite x overflows), and x y = h h + (h m + m h) + (m m + h l + l h), smallest first; what is left out is under 2^-21 of it.
+// fp32 on the bf16 products: x = h + m + l, three bf16 values of 8 bits each, exactly where l is not under the smallest normal
+// number (h and m cut off, no rounding, so that no finite x overflows), and x y = h h + (h m + m h) + (m m + h l + l h), smallest
+// first; what is left out, m l + l m + l l, has the product's sign and is under 2^-21 of it (m < 2^-7 x, l < 2^-15 x): eight half-steps
+// of fp32, where a chain of D fp32 products may lose D.  Calls of at most 32 rows take the fp32 instruction, so the last digits of a
+// row are other ones there.
 // Six products of 2.5 PFLOP/s peak against the 157 TFLOP/s of the fp32 instruction.  An infinity or NaN makes NaN, which the
 // end of the kernel looks for.
 struct Thirds { bf8 h, m, l; };
@@ -488,7 +496,7 @@ __global__ __launch_bounds__(64 * WQ * WK, (Shape<T, NS, NQ, WQ, WK, KB>::WAVES)
         }
     };
     // Weights: fp32 in the sum; rounded to the tensor's type (16-bit) for the product with the values, as the matrix instructions
-    // take them: half a step, 2^-9 or 2^-12 relative, of each weight, next to the same of the result
+    // take them: half a step, 2^-8 or 2^-11 relative, of each weight, next to the same of the result
     auto weights = [&](f32x16 (&sc)[NQ], frag (&pf)[NQ][2]) {
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {

@@ -7,8 +7,10 @@
 //
 // Bound: memory.  A row lives in the registers of the wave or block that owns it, so x (and dy) are read once; a block of the
 // backward pass walks over many rows with its share of dw and db in registers, and a second kernel adds the blocks' shares
-// in a fixed order (no atomics: the same bits every time).  24571 x 4096 bf16: forward 88 us (4.6 TB/s), backward with its sums
-// 115 us (5.2 TB/s); 25120 x 768 fp32: 26 and 43 us (a copy of that size stays in the cache: 6 .. 8 TB/s).
+// in a fixed order (no atomics: the same bits every time).  24571 x 4096 bf16: forward 86 us (4.7 TB/s), backward with its sums
+// 117 us (5.2 TB/s); 25120 x 768 fp32: 25 and 40 us (a copy of that size stays in the cache: 6 .. 8 TB/s).  Widths that 16 bytes do not
+// divide go entry by entry: 24571 x 1001 bf16 39 and 37 us (2.5, 4.0 TB/s), fp32 36 and 56 (5.4); over 16384 entries x is read in
+// passes: 2000 x 32768 bf16 67 and 221 us.
 #include <initializer_list>
 
 #include "common.h"

@@ -4,11 +4,13 @@
 // the pair is (i, i + part/2), in the interleaved one (2i, 2i + 1), counted from `offset`; the rest of the head passes.
 // Cosines and sines: theta and its remainder by pi/2 in fp64 (a position of 4e6 leaves an fp32 angle no digit behind the
 // point), then Taylor polynomials on [-pi/4, pi/4] in fp32 (first dropped terms 7e-12 and 1.2e-10, below half an fp32 step),
-// so the factors are right to fp32 rounding at any position.  They are computed once per token and pair into LDS and used by
-// every head; products and sums are fp32, the result is rounded to the tensor's type once.
+// so the factors are right to fp32 rounding up to angles of 2^28, where the fp64 product's own rounding (2^-53 of the angle) comes to
+// half an fp32 step.  They are computed once per token and pair into LDS and used by every head; products and sums are fp32, the
+// result is rounded to the tensor's type once.
 //
-// Bound: memory; each element is read once and written once, nothing else is of size.  65536 tokens x 40 heads of 128 in bf16
-// (1.34 GB), half of each turning: 238 us, 5.6 TB/s, where a copy of 1 GB reaches 5.2.
+// Bound: memory; each element is read once and written once, nothing else is of size.  131072 tokens x 40 heads of 128 in bf16 (2.7
+// GB) 486 us, 5.5 TB/s; 24571 x 40 in fp16, half of each interleaved, 93 us, 5.4; a copy of 1 GB reaches 5.0.  Narrower accesses cost
+// more: 24 of 128 entries in halves (12 pairs: two entries at a time) 244 us for 24571 x 40.
 #include "common.h"
 
 namespace {

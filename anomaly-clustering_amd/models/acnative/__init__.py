@@ -1101,7 +1101,8 @@ def attention_packed(q, k, v, starts_q, starts_k=None, max_q=None, max_k=None, c
     query i of n sees key j of m where j <= i + m - n.  A row that sees no key, or none with a score above -inf, is zero; rows outside every sequence are left as they
     were in `out` (without `out`: zero).  scale: 1 / sqrt(dim) unless given.  want_sums: also the fp32 [tokens, heads] logarithm of
     each row's sum of exponentials (-inf for a row that sees no key, and outside every sequence).
-    Tensors whose heads do not start at multiples of 16 bytes are copied first."""
+    The bounds choose the launch and with it the last digits of a row (fp32: 2^-21 of each product; at most 32 rows of max_q * heads /
+    kv_heads go by other instructions than more); the same call gives the same bits.  Tensors whose heads do not start at multiples of 16 bytes are copied first."""
     shape, qs = _heads(q, "q")
     tokens, heads, dim = shape
     dtype, device = q.dtype, q.device

@@ -47,11 +47,11 @@ extern "C" {
 #define AC_EWORKSPACE 2 /* workspace too small */
 #define AC_ELAUNCH 3    /* HIP reported a launch error */
 
-/* ABI revision: changes whenever an entry point changes meaning or a new one is added; a binding checks it at load
- * time (models/acnative does: a stale library under a newer binding - or the reverse - fails there, not in a kernel).
- * 500 = round 5: ac_alpha_softmax is the 7-argument form again, the fp32 copy moved to ac_alpha_softmax_f32.
- * 600: ac_patch_aggregate_hl32 / ac_patch_aggregate_hl32_supported added.  The entry points for packed sequences
- * came later and left it: nothing else changed, and a binding that misses one fails on its name. */
+/* ABI revision: changes whenever an entry point or an argument structure changes meaning or layout; a binding checks it at load
+ * time (models/acnative does: a stale library under a newer binding - or the reverse - fails there, not in a kernel).  An entry
+ * point that is only added leaves it (up to 600 an addition raised it too): a binding that misses one fails on its name.
+ * 500: ac_alpha_softmax is the 7-argument form again, the fp32 copy moved to ac_alpha_softmax_f32.
+ * 600: ac_patch_aggregate_hl32 / ac_patch_aggregate_hl32_supported added. */
 #define AC_ABI_VERSION 600
 int ac_version(void);
 const char* ac_last_error(void);
@@ -329,8 +329,7 @@ int ac_cluster_scores(const int32_t* labels_true, const int32_t* labels_pred, in
 /* Operators on sequences of different lengths that lie one behind the other in [tokens, heads, dim] tensors (images of their
  * own sizes, prompts of their own lengths): sequence s is the rows starts[s] .. starts[s + 1].  Strides are in entries, the
  * entries of a head are neighbours.  They need no reference counterpart: the reference's ViT (vision_transformer.py:80-92)
- * takes one length per batch and learned positions.  Adding them left every earlier entry point as it was, and a binding
- * that misses one fails on its name, so AC_ABI_VERSION stays. */
+ * takes one length per batch and learned positions. */
 #define AC_F32 0
 #define AC_F16 1
 #define AC_BF16 2
@@ -359,7 +358,10 @@ int ac_rotary(const ac_rotary_args* args, void* stream);
 /* Attention over packed sequences: out[t, h] = sum_j p_j v[j, g], p = softmax(scale * q[t, h] . k[j, g]) over the keys of the
  * token's own sequence, g = h / (heads / kv_heads).  causal: query i of n sees key j of m where j <= i + m - n (the last query
  * sees every key).  A row that sees no key (or none with a score above -inf) is zero and its log-sum -inf; a key that a
- * row does not see cannot touch it, whatever it holds.  Rows before the first and behind the last sequence are left as they are; clear
+ * row does not see cannot touch it, whatever it holds.  Values that it sees pass as they are, infinities and NaN included, and finite ones of
+ * any size keep their weighted mean.  Products and sums are fp32; 16-bit types round the weights to their type for the product with
+ * v; fp32 goes to 2^-21 of each product, by other instructions for at most 32 rows (max_q * heads / kv_heads), so that the last
+ * digits of a row may differ from launch shape to launch shape, never from call to call.  Rows before the first and behind the last sequence are left as they are; clear
  * & 1 makes them zero in out, clear & 2 -inf in sums.
  * starts_q, starts_k: int32 [sequences + 1] on the device, not decreasing, clamped there to 0 .. tokens.  max_q, max_k: upper bounds of the
  * lengths, used for the launch's shape alone (too small a bound costs time, not rows).  sums (nullable): fp32 [tokens_q,
